@@ -367,6 +367,65 @@ int mgx_unified_encode_tokens(const int* notes, const int* velocities, const int
                               const int* starts, int B, int Nmax, int seq_len, int note_bins, int velocity_bins,
                               int duration_bins, int* tokens, void* stream);
 
+/* ---- rotary positions in every form -----------------------------------------------------------------
+ * Beside mgx_rope_qk (packed projection, interleaved pairs, whole head, positions 0..S-1):
+ *   x, y [B,S,H,dh] with element strides (last one 1), y == x with equal strides rotates in place (rows that overlap,
+ *   or a y that overlaps x in part, are the caller's error); the first rd values of a head are turned, the rest copied
+ *   half_layout 0: pairs (x[2i], x[2i+1])   1: pairs (x[i], x[i + rd/2])       i < rd/2
+ *   y[a] = x[a] cos - x[b] sin, y[b] = x[b] cos + x[a] sin, in fp32; transposed != 0: sin negated (the gradient)
+ *   cos_tab / sin_tab [table_rows, rd/2] fp32; positions [B,S] int32 or int64 (clamped to the table), NULL: row s has s
+ * Any rd, strides and alignment; rows of 16-byte multiples take the wide kernels. */
+int mgx_rotary(const void* x, void* y, const float* cos_tab, const float* sin_tab, const void* positions,
+               int positions_are_int64, int B, int S, int H, int dh, int rd, int table_rows, long xsb, long xss, long xsh,
+               long ysb, long yss, long ysh, int half_layout, int transposed, int dtype, void* stream);
+/* cos_tab, sin_tab [n, half] fp32 = amplitude * cos, sin (position * freq[i]), positions 0..n-1; freq [half] fp64 on the
+ * device.  Angles and their functions in 64 bits. */
+int mgx_rope_tables(const double* freq, float* cos_tab, float* sin_tab, long n, int half, double amplitude, void* stream);
+
+/* ---- a paged K/V cache: filing, attention ---------------------------------------------------------------
+ * Beside mgx_kv_append / mgx_decode_attn (one dense [B,H,Lmax,dh] cache, rows at one common position):
+ *   kcache, vcache [n_pages, Hkv, page, dh]; table [B, width] int32: own key j of sequence b is row j % page of page
+ *   table[b][j / page]; lens [B] int32: own keys of a sequence, the new rows' included
+ *   the T new rows: R for each of the B sequences, or ragged: rows cu_rows[b] .. cu_rows[b+1]-1 (int32, ascending from 0;
+ *   rows behind cu_rows[B] belong to none).  Row r of sequence b has own index lens[b] - n_b + r.
+ * Everything the device holds is checked there: a page outside the pool or an index outside the table files nothing and
+ * is not attended.
+ *
+ * mgx_paged_append: qkv [T, (Hq + 2 Hkv) dh] = q | k | v heads.  k (rotated) and v are filed, q goes to q_out [T,Hq,dh]
+ * rotated (zero for rows of no sequence).  Position = offset + own index (clamped to the table); rd, half_layout as
+ * mgx_rotary.  cos_tab == NULL: nothing is rotated and q_out (may be NULL) not written.  Two rows with the same slot:
+ * one of them stays, which one is not defined. */
+int mgx_paged_append(const void* qkv, void* q_out, void* kcache, void* vcache, const int* table, const int* lens,
+                     const int* cu_rows, const float* cos_tab, const float* sin_tab, long T, int B, int R, int Hq, int Hkv,
+                     int dh, int rd, int page, int n_pages, int width, int table_rows, int offset, int half_layout,
+                     int dtype, void* stream);
+/* mgx_paged_attn: row r of sequence b attends the first prefix_len keys of the pages prefix[] (shared by the whole batch:
+ * their K and V are read once per row tile of the batch, not once per sequence) and its own keys up to its own index;
+ *   out = softmax(scale q.k + slope_h (j - i)) v      i = prefix_len + own index; slopes [Hq] fp32 or NULL
+ * q [T,Hq,dh] with q_row_stride elements from row to row, out [T,Hq,dh]; query head h reads K/V head h / (Hq / Hkv).
+ * A row that sees no key, and a row of no sequence, gets zeros.  What masked slots hold (stale values, NaN) has no
+ * effect.  max_rows / max_len: upper bounds of n_b and lens[b] that shape the launch (wrong ones cost time, not results).
+ * workspace: mgx_paged_attn_workspace_floats floats for the same arguments.  dh <= 256, a multiple of 16 bytes. */
+long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows, int max_len,
+                                     int dtype);
+int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const void* vcache, const int* table,
+                   const int* lens, const int* cu_rows, const float* slopes, const int* prefix, void* out, float* workspace,
+                   long T, int B, int R, int Hq, int Hkv, int dh, int page, int n_pages, int width, int prefix_len,
+                   int max_rows, int max_len, float scale, int dtype, void* stream);
+
+/* ---- verification of drafted tokens ----------------------------------------------------------------------
+ * Beside mgx_sample_head: speculative sampling from given uniforms in [0, 1).
+ *   target [B,k+1,V], draft [B,k,V] probabilities (element strides of batch and row; classes contiguous), tokens [B,k]
+ *   (the draft's, int32 or int64), uniforms [B,k+1], counts [B] int32 (tokens drafted, NULL: k)
+ *   token i stays while u_i q_i(x_i) < p_i(x_i); behind the a that stay one token is drawn with u_k from max(p_a - q_a, 0),
+ *   or from p_a when all stayed (or nothing is left over): the smallest class whose running sum passes u_k * total
+ *   out [B,k+1] (as tokens): the tokens that stay, the drawn one, -1 behind; accepted [B] int32 = a
+ *   draft == NULL: drafted tokens were certain (q = one-hot).  Values that are not positive and finite weigh nothing.
+ * Products and running sums in fp64, fixed order. */
+int mgx_verify_draft(const void* target, const void* draft, const void* tokens, int tokens_are_int64, const float* uniforms,
+                     const int* counts, void* out, int* accepted, int B, int k, long V, long target_stride_b,
+                     long target_stride_row, long draft_stride_b, long draft_stride_row, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

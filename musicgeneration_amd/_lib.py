@@ -18,6 +18,7 @@ GENERIC_KERNELS = 0x100        # OR-ed into an attention call's dtype: generic k
 ACT_GELU, ACT_RELU = 0, 1
 
 _vp, _i, _l, _f, _u64, _ll = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_ulonglong, C.c_longlong
+_d = C.c_double
 
 PROTOTYPES = {
     "mgx_version": (C.c_int, []),
@@ -70,6 +71,12 @@ PROTOTYPES = {
     "mgx_gemm_tn_workspace_floats": (_l, [_i, _i, _i, _vp]),
     "mgx_gemm_tn_bf16": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "mgx_gemm_tn_pair_workspace_floats": (_l, [_i, _i, _i, _i, _i]),
+    "mgx_rotary": (_i, [_vp] * 5 + [_i] * 7 + [_l] * 6 + [_i, _i, _i, _vp]),
+    "mgx_rope_tables": (_i, [_vp, _vp, _vp, _l, _i, _d, _vp]),
+    "mgx_paged_append": (_i, [_vp] * 9 + [_l] + [_i] * 13 + [_vp]),
+    "mgx_paged_attn_workspace_floats": (_l, [_l] + [_i] * 8),
+    "mgx_paged_attn": (_i, [_vp, _l] + [_vp] * 9 + [_l] + [_i] * 11 + [_f, _i, _vp]),
+    "mgx_verify_draft": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _l, _l, _l, _l, _l, _i, _vp]),
     "mgx_gemm_tn_pair_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp]),
 }
 

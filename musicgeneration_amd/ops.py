@@ -1160,3 +1160,361 @@ def adamw_step_multi(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps
     with _timed("adamw", 28.0 * sum(p.numel() for p in params)):       # p, m, v read + written, g read: 28 B per parameter
         check(lib.mgx_adamw_multi(n, arr(params), arr(grads), arr(exp_avgs), arr(exp_avg_sqs), sizes, lr, beta1, beta2, eps,
                                   weight_decay, step, grad_scale, _stream()), "mgx_adamw_multi")
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+_HALF = {"interleaved": 0, "half": 1}
+
+
+def _on(device, launch):
+    """launch(stream) with `device` current: its current stream is where the tensors' work belongs."""
+    if device.index == torch.cuda.current_device():
+        return launch(torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return launch(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _beside(t, name, like, dtypes):
+    """A dense tensor of one of `dtypes` on the device of `like`."""
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {like.device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+_FP32, _INT32, _INTS = (torch.float32,), (torch.int32,), (torch.int32, torch.int64)
+
+
+def _rope_tables_ok(cos, sin, dh, like, name):
+    _beside(cos, "cos", like, _FP32)
+    _beside(sin, "sin", like, _FP32)
+    if cos.dim() != 2 or cos.shape != sin.shape or not 0 < 2 * cos.shape[1] <= dh or cos.shape[0] == 0:
+        raise ValueError(f"{name}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [positions, rd/2], rd <= {dh}")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError(f"{name}: no gradient is formed for cos and sin")
+
+
+def rope_tables(n: int, rotary_dim: int, base: float = 10000.0, scaling=None, factor: float = 1.0, original: int = 0,
+                device="cuda"):
+    """(cos, sin) [n, rotary_dim/2] fp32 for positions 0..n-1; angles and their functions are taken in 64 bits.
+
+    scaling, for contexts `factor` times longer than trained:
+      None        theta_i = base^(-2i/rd)
+      "linear"    theta_i / factor (positions interpolated)
+      "ntk"       base * factor^(rd/(rd-2)): the slowest pair is interpolated by `factor`, the fastest not at all
+      "by_parts"  pairs that turn more than 32 times over the `original` trained length stay, those that turn less than
+                  once are interpolated, a linear ramp between; cos and sin are scaled by 1 + 0.1 ln(factor)
+    """
+    if n < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rope_tables: n={n} rotary_dim={rotary_dim}")
+    if not base > 1.0 or not 1.0 <= factor < math.inf:
+        raise ValueError(f"rope_tables: base {base} must exceed 1 and factor {factor} be a finite number of at least 1")
+    amplitude = 1.0
+    half = rotary_dim // 2
+    theta = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+    if scaling == "linear":
+        theta = [t / factor for t in theta]
+    elif scaling == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("rope_tables: ntk scaling needs rotary_dim of at least 4")
+        longer = base * factor ** (rotary_dim / (rotary_dim - 2.0))
+        theta = [longer ** (-2.0 * i / rotary_dim) for i in range(half)]
+    elif scaling == "by_parts":
+        if original < 1:
+            raise ValueError("rope_tables: by_parts scaling needs the original length")
+        keep = [min(max((original * t / (2.0 * math.pi) - 1.0) / 31.0, 0.0), 1.0) for t in theta]
+        theta = [t * (k + (1.0 - k) / factor) for t, k in zip(theta, keep)]
+        amplitude = 1.0 + 0.1 * math.log(factor)
+    elif scaling is not None:
+        raise ValueError(f"rope_tables: scaling {scaling!r} (None, 'linear', 'ntk', 'by_parts')")
+    freq = torch.tensor(theta, dtype=torch.float64).to(device)
+    if not freq.is_cuda:
+        raise RuntimeError("rope_tables: musicgeneration_amd runs on the GPU only; there is no CPU fallback")
+    cos = torch.empty(n, half, dtype=torch.float32, device=freq.device)
+    sin = torch.empty_like(cos)
+    check(_on(freq.device, lambda st: lib.mgx_rope_tables(_p(freq), _p(cos), _p(sin), n, half, amplitude, st)),
+          "mgx_rope_tables")
+    return cos, sin
+
+
+def _rotary(x, y, cos, sin, positions, half, transposed):
+    B, S, H, dh = x.shape
+    if B * S * H == 0:
+        return y
+    xs, ys = x.stride(), y.stride()
+    check(_on(x.device, lambda st: lib.mgx_rotary(
+        x.data_ptr(), y.data_ptr(), cos.data_ptr(), sin.data_ptr(), _p(positions),
+        0 if positions is None or positions.dtype == torch.int32 else 1, B, S, H, dh, 2 * cos.shape[1], cos.shape[0],
+        xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], half, transposed, _dt(x), st)), "mgx_rotary")
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    """Linear in x: its gradient is the transposed rotation of the incoming one (and so on, to any order)."""
+
+    @staticmethod
+    def forward(ctx, x, cos, sin, positions, half, transposed):
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.cfg = half, transposed
+        return _rotary(x, torch.empty(x.shape, dtype=x.dtype, device=x.device), cos, sin, positions, half, transposed)
+
+    @staticmethod
+    def backward(ctx, dy):
+        cos, sin, positions = ctx.saved_tensors
+        half, transposed = ctx.cfg
+        if dy.stride(-1) != 1:
+            dy = dy.contiguous()
+        return _Rotary.apply(dy, cos, sin, positions, half, 1 - transposed), None, None, None, None, None
+
+
+def _rotary_args(x, cos, sin, positions, layout, name):
+    if not x.is_cuda:
+        raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (x is on {x.device}); there is no CPU fallback")
+    _dt(x)
+    if x.dim() != 4 or x.shape[3] < 2 or x.stride(3) != 1:
+        raise ValueError(f"{name}: x {tuple(x.shape)} must be [batch, seq, heads, dh] with unit stride in dh")
+    if layout not in _HALF:
+        raise ValueError(f"{name}: layout {layout!r} ('interleaved', 'half')")
+    B, S, H, dh = x.shape
+    if dh % 2 and layout == "interleaved":
+        raise ValueError(f"{name}: the interleaved layout needs an even head dim, got {dh}")
+    _rope_tables_ok(cos, sin, dh, x, name)
+    if positions is None:
+        if S > cos.shape[0]:
+            raise ValueError(f"{name}: {S} rows, tables of {cos.shape[0]} positions")
+    else:
+        _beside(positions, "positions", x, _INTS)
+        if positions.shape != (B, S):
+            raise ValueError(f"{name}: positions {tuple(positions.shape)} must be {(B, S)}")
+    return _HALF[layout]
+
+
+def rotary(x, cos, sin, positions=None, layout: str = "interleaved"):
+    """Rotary positions of x [B,S,H,dh] (any strides, unit stride in dh: the q | k heads of a packed projection are one
+    view): a new dense tensor; differentiable in x.
+
+    cos, sin [P, rd/2] fp32 (rope_tables); the first rd <= dh values of a head are turned, the rest copied.
+    layout: "interleaved" pairs (2i, 2i+1), "half" pairs (i, i + rd/2).
+    positions [B,S] int32 / int64, None: 0..S-1.  Positions outside the tables are clamped to their ends."""
+    half = _rotary_args(x, cos, sin, positions, layout, "rotary")
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, cos, sin, positions, half, 0)
+    return _rotary(x, torch.empty(x.shape, dtype=x.dtype, device=x.device), cos, sin, positions, half, 0)
+
+
+def _overlaps(x) -> bool:
+    """Whether two elements of x may share memory (a broadcast dimension, windows)."""
+    reach = 0
+    for stride, size in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
+        if stride <= reach:
+            return True
+        reach += stride * (size - 1)
+    return False
+
+
+def rotary_(x, cos, sin, positions=None, layout: str = "interleaved", transposed: bool = False):
+    """rotary in place, outside autograd; transposed=True applies the gradient's rotation."""
+    half = _rotary_args(x, cos, sin, positions, layout, "rotary_")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotary_ is not seen by autograd: use rotary, or torch.no_grad()")
+    if _overlaps(x):
+        raise ValueError("rotary_: elements of x share memory")
+    return _rotary(x, x, cos, sin, positions, half, 1 if transposed else 0)
+
+
+# ---------------------------------------------------------------------------
+# paged K/V cache: filing, attention over a shared prefix and own pages; verification of drafted tokens
+# ---------------------------------------------------------------------------
+def _no_grad_of(name, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{name} forms no gradient: call it under torch.no_grad()")
+
+
+def _cache_args(kcache, vcache, table, lens, like, name):
+    for t, what in ((kcache, "kcache"), (vcache, "vcache")):
+        _beside(t, what, like, (like.dtype,))
+        if t.data_ptr() % 16:
+            raise ValueError(f"{name}: {what} must be 16-byte aligned")
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.numel() == 0 or kcache.data_ptr() == vcache.data_ptr():
+        raise ValueError(f"{name}: kcache {tuple(kcache.shape)} and vcache {tuple(vcache.shape)} must be two "
+                         "[pages, heads, page, dh] pools")
+    n_pages, Hkv, page, dh = kcache.shape
+    if dh % (16 // kcache.element_size()) or dh > 256:
+        raise ValueError(f"{name}: head dim {dh} must be a multiple of {16 // kcache.element_size()} up to 256")
+    _beside(table, "table", like, _INT32)
+    _beside(lens, "lens", like, _INT32)
+    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0] or table.numel() == 0:
+        raise ValueError(f"{name}: table {tuple(table.shape)} must be [sequences, pages], lens {tuple(lens.shape)} [sequences]")
+    return n_pages, Hkv, page, dh
+
+
+def _cu_args(cu_rows, lens, like, name):
+    _beside(cu_rows, "cu_rows", like, _INT32)
+    if cu_rows.dim() != 1 or cu_rows.shape[0] != lens.shape[0] + 1:
+        raise ValueError(f"{name}: cu_rows {tuple(cu_rows.shape)} must hold {lens.shape[0] + 1} offsets")
+
+
+def paged_append(qkv, kcache, vcache, table, lens, n_heads: int, cos=None, sin=None, layout: str = "interleaved",
+                 cu_rows=None, offset: int = 0):
+    """File the new rows' k (rotated) and v in a paged cache and return their rotated q.
+
+    qkv [B,R,(Hq+2*Hkv)*dh] (R new rows for each sequence), or [T,...] with cu_rows [B+1] int32 (sequence b has rows
+    cu_rows[b]..cu_rows[b+1]-1; rows behind the last sequence file nothing); n_heads = Hq.
+    kcache, vcache [pages, Hkv, page, dh]; table [B, width] int32 page numbers; lens [B] int32 = own keys of each
+    sequence, the new rows included.  Own index of row r: lens[b] - n_b + r; its position: offset + own index (offset =
+    the shared prefix's length).  cos, sin, layout as `rotary`; None: no rotation, q comes back as a view of qkv.
+    A page number outside the pool and an index outside the table file nothing.  Returns q [B,R,Hq,dh] or [T,Hq,dh]."""
+    name = "paged_append"
+    if not qkv.is_cuda:
+        raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (qkv is on {qkv.device}); there is no CPU fallback")
+    _dt(qkv)
+    _no_grad_of(name, qkv)
+    if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+        raise ValueError(f"{name}: qkv must be contiguous and 16-byte aligned")
+    n_pages, Hkv, page, dh = _cache_args(kcache, vcache, table, lens, qkv, name)
+    B, width = table.shape
+    if n_heads < 1 or qkv.dim() != (3 if cu_rows is None else 2) or qkv.shape[-1] != (n_heads + 2 * Hkv) * dh or \
+            (cu_rows is None and qkv.shape[0] != B):
+        raise ValueError(f"{name}: qkv {tuple(qkv.shape)} for {B} sequences, {n_heads} + 2 x {Hkv} heads of {dh}"
+                         f"{'' if cu_rows is None else ', ragged'}")
+    if cu_rows is not None:
+        _cu_args(cu_rows, lens, qkv, name)
+    if layout not in _HALF:
+        raise ValueError(f"{name}: layout {layout!r} ('interleaved', 'half')")
+    if not 0 <= offset < 2 ** 30:
+        raise ValueError(f"{name}: offset {offset}")
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{name}: cos and sin go together")
+    lead = qkv.shape[:-1]
+    T = lead.numel()
+    if cos is None:
+        q = qkv[..., :n_heads * dh].unflatten(-1, (n_heads, dh))
+        q_ptr = rd = rows = 0
+    else:
+        _rope_tables_ok(cos, sin, dh, qkv, name)
+        q = torch.empty(*lead, n_heads, dh, dtype=qkv.dtype, device=qkv.device)
+        q_ptr, rows, rd = q.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+    if T:
+        check(_on(qkv.device, lambda st: lib.mgx_paged_append(
+            qkv.data_ptr(), q_ptr, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows),
+            _p(cos), _p(sin), T, B, 0 if cu_rows is not None else lead[1], n_heads, Hkv, dh, rd, page, n_pages, width, rows,
+            offset, _HALF[layout], _dt(qkv), st)), "mgx_paged_append")
+    return q
+
+
+def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_rows: Optional[int] = None,
+               max_len: Optional[int] = None, prefix=None, prefix_len: int = 0, scale: Optional[float] = None):
+    """Attention of the new rows over a prefix that the whole batch shares and each sequence's own paged keys.
+
+    q [B,R,Hq,dh], or [T,Hq,dh] with cu_rows (as paged_append; a row stride of its own is fine: the q heads of a packed
+    projection); kcache, vcache, table, lens as paged_append, after it.  prefix: int32 page numbers of the shared prefix in
+    the same pool, prefix_len its keys (its K and V are read once for the batch, not once for each sequence).
+    Row r of sequence b stands at i = prefix_len + lens[b] - n_b + r and sees the prefix and its own keys up to itself:
+    softmax(scale * q.k + slope_h * (j - i)) v; slopes [Hq] fp32 (ALiBi) or None; scale defaults to dh^-1/2.
+    Hq a multiple of Hkv: query head h reads head h // (Hq // Hkv).  Rows that see nothing get zeros; what masked slots
+    hold has no effect.  max_rows, max_len: upper bounds of n_b and lens[b], known on the host, that shape the launch
+    (defaults: all rows, the table's width; a wrong one costs time, not results).  Returns a dense tensor of q's shape."""
+    name = "paged_attn"
+    if not q.is_cuda:
+        raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (q is on {q.device}); there is no CPU fallback")
+    _dt(q)
+    _no_grad_of(name, q, slopes)
+    n_pages, Hkv, page, dh = _cache_args(kcache, vcache, table, lens, q, name)
+    B, width = table.shape
+    if q.dim() != (4 if cu_rows is None else 3) or q.shape[-1] != dh or (cu_rows is None and q.shape[0] != B):
+        raise ValueError(f"{name}: q {tuple(q.shape)} for {B} sequences, heads of {dh}{'' if cu_rows is None else ', ragged'}")
+    Hq = q.shape[-2]
+    if Hq == 0 or Hq % Hkv or Hq > 65535:
+        raise ValueError(f"{name}: {Hq} query heads over {Hkv} key heads")
+    if cu_rows is not None:
+        _cu_args(cu_rows, lens, q, name)
+    if slopes is not None:
+        _beside(slopes, "slopes", q, _FP32)
+        if slopes.shape != (Hq,):
+            raise ValueError(f"{name}: slopes {tuple(slopes.shape)} for {Hq} heads")
+    if prefix_len:
+        if prefix is None or prefix_len < 0:
+            raise ValueError(f"{name}: prefix_len {prefix_len}, prefix {None if prefix is None else tuple(prefix.shape)}")
+        _beside(prefix, "prefix", q, _INT32)
+        if prefix.dim() != 1 or prefix_len > prefix.shape[0] * page:
+            raise ValueError(f"{name}: {prefix_len} prefix keys in pages {tuple(prefix.shape)} of {page}")
+    if page * width + prefix_len >= 2 ** 30:
+        raise ValueError(f"{name}: tables of {page * width} keys behind {prefix_len}")
+    scale = dh ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{name}: scale {scale}")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    T = out.numel() // (Hq * dh)
+    if T == 0:
+        return out
+    R = 0 if cu_rows is not None else q.shape[1]
+    max_rows = R or min(T, T if max_rows is None else max_rows)
+    max_len = page * width if max_len is None else min(max_len, page * width)
+    if max_rows < 1 or max_len < 0:
+        raise ValueError(f"{name}: max_rows {max_rows}, max_len {max_len}")
+    # one row stride over the whole batch, heads dense inside a row
+    st = q.stride()
+    if cu_rows is None:
+        row = st[1] if R > 1 else st[0] if B > 1 else Hq * dh
+        flat = R == 1 or B == 1 or st[0] == R * st[1]
+    else:
+        row, flat = st[0] if T > 1 else Hq * dh, True
+    if not flat or st[-1] != 1 or (st[-2] != dh and Hq > 1) or row < Hq * dh or row % (16 // q.element_size()) or q.data_ptr() % 16:
+        q, row = q.contiguous(), Hq * dh
+        if q.data_ptr() % 16:
+            q = q.clone()
+    dt = _dt(q)
+    floats = lib.mgx_paged_attn_workspace_floats(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dt)
+    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    check(_on(q.device, lambda s: lib.mgx_paged_attn(
+        q.data_ptr(), row, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows), _p(slopes),
+        _p(prefix) if prefix_len else None, out.data_ptr(), _p(ws), T, B, R, Hq, Hkv, dh, page, n_pages, width, prefix_len,
+        max_rows, max(max_len, 1), scale, dt, s)), "mgx_paged_attn")
+    return out
+
+
+def verify_draft(target, tokens, uniforms, draft=None, counts=None):
+    """Verify drafted tokens against the target model's probabilities (speculative sampling) from given uniforms.
+
+    target [B,k+1,V] probabilities of the k drafted positions and the one behind (rows may be padded: a [..., :V] view);
+    tokens [B,k] int32 / int64; uniforms [B,k+1] fp32 in [0, 1); draft [B,k,V] probabilities the tokens were drawn from,
+    None: they were certain; counts [B] int32: tokens drafted per sequence, None: k.
+    Token i stays while u_i q_i(x_i) < p_i(x_i).  Behind the a tokens that stay, one is drawn with uniforms[:, k] from
+    max(p_a - q_a, 0), or from p_a when all stayed (or nothing is left over): the smallest class whose running sum (fp64)
+    passes u * total.  Probabilities that are not positive and finite weigh nothing; a drafted class outside [0, V) does
+    not stay.  Returns (out [B,k+1] as tokens: those that stay, the drawn one, -1 behind; accepted [B] int32 = a)."""
+    name = "verify_draft"
+    if not target.is_cuda:
+        raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (target is on {target.device}); there is no CPU fallback")
+    dt = _dt(target)
+    _no_grad_of(name, target, draft)
+    if target.dim() != 3 or target.shape[1] < 1 or not 0 < target.shape[2] < 2 ** 31 or \
+            (target.stride(2) != 1 and target.shape[2] > 1):
+        raise ValueError(f"{name}: target {tuple(target.shape)} must be [batch, drafts + 1, classes], classes contiguous")
+    B, k, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    _beside(tokens, "tokens", target, _INTS)
+    _beside(uniforms, "uniforms", target, _FP32)
+    if tokens.shape != (B, k) or uniforms.shape != (B, k + 1):
+        raise ValueError(f"{name}: tokens {tuple(tokens.shape)} and uniforms {tuple(uniforms.shape)} for {B} x {k} drafts")
+    if draft is not None:
+        if draft.device != target.device or draft.dtype != target.dtype:
+            raise TypeError(f"{name}: draft {draft.dtype} on {draft.device}, target {target.dtype} on {target.device}")
+        if draft.shape != (B, k, V) or (draft.stride(2) != 1 and V > 1):
+            raise ValueError(f"{name}: draft {tuple(draft.shape)} must be {(B, k, V)}, classes contiguous")
+    if counts is not None:
+        _beside(counts, "counts", target, _INT32)
+        if counts.shape != (B,):
+            raise ValueError(f"{name}: counts {tuple(counts.shape)} must be {(B,)}")
+    out = torch.empty(B, k + 1, dtype=tokens.dtype, device=target.device)
+    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
+    if B:
+        ds = draft.stride() if draft is not None else (0, 0)
+        check(_on(target.device, lambda st: lib.mgx_verify_draft(
+            target.data_ptr(), _p(draft) if k else None, _p(tokens), 1 if tokens.dtype == torch.int64 else 0,
+            uniforms.data_ptr(), _p(counts), out.data_ptr(), accepted.data_ptr(), B, k, V, target.stride(0),
+            target.stride(1), ds[0], ds[1], dt, st)), "mgx_verify_draft")
+    return out, accepted

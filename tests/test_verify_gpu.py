@@ -1,0 +1,95 @@
+"""verify_draft (mgx_verify_draft) against the 64-bit loop of serving_oracle: whole numbers, so exactly equal."""
+import pytest
+import torch
+
+from serving_oracle import verify
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(B, k, V, dtype, seed, agree=0.7, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    logits = 2 * torch.randn(B, k + 1, V, generator=g)
+    q = (agree * logits[:, :k] + 2 * (1 - agree) * torch.randn(B, k, V, generator=g)).softmax(-1)
+    tokens = torch.multinomial(q.reshape(B * k, V), 1, generator=g).view(B, k) if k else torch.zeros(B, 0, dtype=torch.int64)
+    wide = lambda p: torch.nn.functional.pad(p.to(dtype), (0, pad), value=9.0)   # noqa: E731  (what is behind V is not read)
+    return wide(logits.softmax(-1)), wide(q), tokens, torch.rand(B, k + 1, generator=g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,k,V,pad", [(1, 1, 1, 0), (5, 4, 618, 22), (3, 0, 77, 1), (7, 3, 2, 0), (2, 70, 65, 3), (9, 5, 5001, 0),
+                                       (4, 2, 50257, 7)])
+def test_verify_draft_is_the_loop(dtype, B, k, V, pad):
+    from musicgeneration_amd import ops
+    p, q, x, u = _case(B, k, V, dtype, 17 * V + k, pad=pad)
+    counts = torch.randint(-1, k + 2, (B,), generator=torch.Generator().manual_seed(1)).int()
+    for draft in (q, None):
+        for cnt in (None, counts):
+            for t in (x, x.int()):
+                want, acc = verify(p[..., :V], t, u, None if draft is None else draft[..., :V], cnt)
+                got, n = ops.verify_draft(p.cuda()[..., :V], t.cuda(), u.cuda(),
+                                          None if draft is None else draft.cuda()[..., :V], None if cnt is None else cnt.cuda())
+                assert got.dtype == t.dtype and torch.equal(n.cpu(), acc) and torch.equal(got.cpu(), want)
+
+
+def test_verify_draft_borders():
+    """Dyadic probabilities: sums are exact, so draws that fall exactly on a border are decided, not rounded."""
+    from musicgeneration_amd import ops
+    V = 64
+    p = torch.zeros(8, 2, V)
+    p[:, 0, 3], p[:, 0, 5], p[:, 0, 60] = 0.25, 0.25, 0.5
+    p[:, 1, 0], p[:, 1, 63] = 0.5, 0.5
+    q = torch.zeros(8, 1, V)
+    q[:, 0, 3], q[:, 0, 7] = 0.5, 0.5
+    x = torch.tensor([[3], [3], [3], [7], [3], [-1], [64], [3]])
+    u = torch.tensor([[0.5, 0.0], [0.499, 0.5], [0.75, 1 / 3], [0.0, 0.99], [0.0, 0.4999], [0.0, 0.0], [0.0, 0.9], [0.5, 1.0 - 2.0 ** -24]])
+    want, acc = verify(p, x, u, q)
+    got, n = ops.verify_draft(p.cuda(), x.cuda(), u.cuda(), q.cuda())
+    assert n.tolist() == acc.tolist() == [0, 1, 0, 0, 1, 0, 0, 0]
+    assert torch.equal(got.cpu(), want)
+    assert got[0].tolist() == [5, -1] and got[1].tolist() == [3, 63] and got[4].tolist() == [3, 0]
+
+
+def test_verify_draft_degenerate_rows():
+    """Nothing left over (p <= q everywhere) draws from p; weights that are not positive and finite weigh nothing; a row
+    without weight gives class 0."""
+    from musicgeneration_amd import ops
+    nan, inf = float("nan"), float("inf")
+    p = torch.tensor([[[0.5, 0.5, 0.0], [1.0, 0.0, 0.0]], [[nan, -1.0, 0.25], [0.0, 0.0, 0.0]], [[0.0, 0.0, 0.0], [0.0, 1.0, 0.0]],
+                      [[inf, 0.25, 0.25], [0.0, 0.0, 1.0]], [[0.1, 0.2, nan], [nan, nan, nan]]])
+    q = torch.tensor([[[0.75, 0.75, 0.5]], [[0.0, 0.0, 0.0]], [[1.0, 0.0, 0.0]], [[0.0, 1.0, 0.0]], [[0.0, nan, inf]]])
+    x = torch.tensor([[0], [0], [0], [1], [0]])
+    u = torch.tensor([[0.9, 0.6], [0.1, 0.5], [0.5, 0.5], [0.9, 0.0], [0.5, 0.7]])
+    want, acc = verify(p, x, u, q)
+    got, n = ops.verify_draft(p.cuda(), x.cuda(), u.cuda(), q.cuda())
+    assert torch.equal(n.cpu(), acc) and torch.equal(got.cpu(), want)
+
+
+def test_verify_draft_keeps_the_targets_distribution():
+    """Speculative sampling leaves the target's distribution: over every u on a fine grid, the first token's frequencies
+    are p's.  q has 4 classes of mass 1/4; 4 x 64 x 64 draws, frequencies off by at most the grid's two steps."""
+    from musicgeneration_amd import ops
+    G = 64
+    p = torch.tensor([0.5, 0.125, 0.25, 0.125])
+    grid = (torch.arange(G) + 0.5) / G
+    x, ua, ub = (t.reshape(-1) for t in torch.meshgrid(torch.arange(4.0), grid, grid, indexing="ij"))
+    B = x.numel()
+    got, _ = ops.verify_draft(p.expand(B, 2, 4).contiguous().cuda(), x[:, None].long().cuda(), torch.stack((ua, ub), 1).cuda(),
+                              torch.full((B, 1, 4), 0.25, device="cuda"))
+    freq = torch.bincount(got[:, 0].cpu(), minlength=4).double() / B
+    assert float((freq - p.double()).abs().max()) <= 2.0 / G
+
+
+def test_verify_draft_replays_in_a_graph():
+    from musicgeneration_amd import ops
+    p, q, x, u = (t.cuda() for t in _case(6, 4, 618, torch.float32, 3))
+    ops.verify_draft(p, x, u, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, acc = ops.verify_draft(p, x, u, q)
+    for step in range(4):
+        u.copy_(torch.rand(6, 5, generator=torch.Generator().manual_seed(step)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, n = verify(p.cpu(), x.cpu(), u.cpu(), q.cpu())
+        assert torch.equal(out.cpu(), want) and torch.equal(acc.cpu(), n)
