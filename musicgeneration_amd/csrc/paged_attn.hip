@@ -5,7 +5,19 @@
 //   out = sum_j softmax_j(scale q.k_j + slope_h (j - i)) v_j          zeros where there is no key to see
 //   Key j of the prefix is row j % page of page prefix[j / page], own key j that of page table[b][j / page]; a page outside
 //   the pool hides its keys.  Softmax statistics and sums are fp32.
-#include "mgx_common.h"
+//
+// Keys are numbered through, the prefix's 0..P-1 first.  A work item is (rows, key range): up to 32 or 128 of the rows
+// that read one K/V head - the G = Hq / Hkv query heads of a group are rows of the same tile - against a range of keys.
+//   own items     rows of one sequence, its own keys (all keys, where the prefix is not taken apart)
+//   prefix items  rows of the WHOLE batch, prefix keys: K and V of the prefix are read once per row tile of the batch
+// Every product is arranged as K . Q^T and V^T . P^T on 32x32 MFMA tiles: the row (query) is on the lane, so a row's
+// maximum and sum need one exchange between half-waves per tile, and P goes from the first product's accumulators to the
+// second's operand without leaving the registers.  Two bodies in one launch:
+//   private  <= 32 rows: memory bound.  The four waves take alternate 32-key tiles, each through LDS of its own with the
+//            next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
+//   shared   <= 128 rows, 32 a wave: 64-key tiles in LDS, double buffered, shared by the four waves.
+// Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
+#include "attn_mfma_common.h"
 
 namespace {
 
@@ -14,9 +26,12 @@ struct PagedArgs {
     void* out;
     const int *table, *lens, *cu, *prefix;
     const float* slopes;
-    int B, R, Hq, Hkv, dh, page, n_pages, width, P, max_rows, max_len;
+    float *acc, *ml;                              // joined later: [split][row][dh] sums, [split][row][2] maximum (log2), sum
+    int B, R, Hq, Hkv, dh, page, shift, n_pages, width, P;
     long T, qs;                                   // rows, elements from one row of q to the next
     float scale;
+    // plan
+    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, n_items_p;
 };
 
 // sequence, row in it, rows of it, whether row t belongs to one
@@ -39,7 +54,645 @@ __device__ __forceinline__ bool find_row(const PagedArgs& a, long t, int& b, int
     return r >= 0 && r < n;
 }
 
-// One workgroup of 4 waves per (row, head); a key row is spread over lpr lanes, 16 bytes each.
+constexpr unsigned NONE = 0xFFFFFFFFu;
+constexpr float NEG = -1.0e30f;       // a running maximum before any key: finite, so differences stay numbers
+
+// Where numbered key j of sequence table `own` lies, in rows of the pool; NONE: nowhere (hidden, or not before `end`).
+__device__ __forceinline__ unsigned key_row(const PagedArgs& a, const int* own, int hk, int j, int end) {
+    if (j >= end) return NONE;
+    const bool pre = j < a.P;
+    const int jj = pre ? j : j - a.P;
+    const int p = a.shift >= 0 ? jj >> a.shift : jj / a.page;
+    const unsigned pg = (unsigned)(pre ? a.prefix[p] : own[p]);
+    return pg < (unsigned)a.n_pages ? (pg * a.Hkv + hk) * a.page + (jj - p * a.page) : NONE;
+}
+
+// ---- LDS images and matrix products per storage type ------------------------------------------------------------------
+template <typename T, int DH> struct Prod;
+
+template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; image of attn_mfma_common.h
+    static constexpr int CH = DH / 8;             // 16-byte chunks per row
+    static constexpr int KB = 32 * DH * 2, VB = KB;           // bytes of 32 rows
+    typedef bf16x8 QFrag;
+    static constexpr int NQ = DH / 16;
+    const LaneAddr<DH> la;
+    __device__ __forceinline__ Prod(int lane) : la(lane) {}
+    // which 16-byte piece of 8 rows x 8 chunks a lane moves: eight consecutive lanes - the unit a ds_write_b128 is serviced
+    // in - take four chunks of two rows, 2 x 64 bytes on different banks
+    __device__ static __forceinline__ void piece(int lane, int& row, int& ch) {
+        row = 2 * (lane >> 4) + ((lane >> 2) & 1);
+        ch = (lane & 3) | ((lane >> 1) & 4);
+    }
+    __device__ static __forceinline__ int koff(int row, int ch) { return Img<DH>::off(row, ch); }
+    __device__ static __forceinline__ int voff(int row, int ch) { return Img<DH>::off(row, ch); }
+    __device__ static __forceinline__ int qchunk(int ks, int h5) { return 2 * ks + h5; }
+    __device__ __forceinline__ f32x16 scores(const char* K, const QFrag (&q)[NQ], f32x16 s) const {
+#pragma unroll
+        for (int ks = 0; ks < NQ; ++ks)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read16(K + la.row_read(0, ks)), q[ks], s, 0, 0, 0);
+        return s;
+    }
+    // P is rounded to bf16 for the product (2^-8 relative each, signs independent); its sum is taken before that
+    __device__ __forceinline__ void weigh(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+            const bf16x8 pf = pack8(p, 8 * s2);
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    lds_read_tr_pair(V + la.tr_read(0, s2, 0, d), V + la.tr_read(0, s2, 1, d)), pf, o[d], 0, 0, 0);
+        }
+    }
+    // weigh, where some V value is not finite: such values are left out, and a second product of P with their places (1
+    // there, 0 elsewhere) tells which rows give them weight: those become NaN there, the other rows never meet 0 x inf
+    __device__ __forceinline__ void weigh_odd(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d) {
+            f32x16 z;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = 0.f;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const bf16x8 pf = pack8(p, 8 * s2);
+                bf16x8 vf = lds_read_tr_pair(V + la.tr_read(0, s2, 0, d), V + la.tr_read(0, s2, 1, d)), at;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const bf16_t x = vf[k];            // (bit_cast of a vector-element lvalue reads element 0)
+                    const bool bad = (__builtin_bit_cast(unsigned short, x) & 0x7F80) == 0x7F80;
+                    at[k] = (bf16_t)(bad ? 1.f : 0.f);
+                    vf[k] = bad ? (bf16_t)0.f : x;
+                }
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
+                z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at, pf, z, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = z[r] > 0.f ? __builtin_nanf("") : o[d][r];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __device__ static __forceinline__ bool not_finite(const f32x4& x) {
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned w = __float_as_uint(x[k]);
+            bad |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+        }
+        return bad;
+    }
+};
+
+template <int DH> struct Prod<float, DH> {        // v_mfma_f32_32x32x2_f32: the parity mode, products exact to fp32
+    static constexpr int CH = DH / 4;
+    static constexpr int VS = DH + 8;             // V row stride: rows 4 apart (the two half-waves) lie 32 banks apart
+    static constexpr int KB = 32 * DH * 4, VB = 32 * VS * 4;
+    typedef f32x4 QFrag;
+    static constexpr int NQ = DH / 8;
+    const int l31, h5;
+    __device__ __forceinline__ Prod(int lane) : l31(lane & 31), h5(lane >> 5) {}
+    __device__ static __forceinline__ void piece(int lane, int& row, int& ch) { row = lane >> 3, ch = lane & 7; }
+    __device__ static __forceinline__ int koff(int row, int ch) { return row * DH * 4 + 16 * (ch ^ (row & 15)); }
+    __device__ static __forceinline__ int voff(int row, int ch) { return row * VS * 4 + 16 * ch; }
+    // the reduced index may be taken in any order: half-wave h5 owns chunk 2 c + h5, four steps of one value each
+    __device__ static __forceinline__ int qchunk(int ks, int h) { return 2 * ks + h; }
+    __device__ __forceinline__ f32x16 scores(const char* K, const QFrag (&q)[NQ], f32x16 s) const {
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            const f32x4 k = *reinterpret_cast<const f32x4*>(K + koff(l31, 2 * c + h5));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[c][e], s, 0, 0, 0);
+        }
+        return s;
+    }
+    __device__ __forceinline__ void weigh(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float* v = reinterpret_cast<const float*>(V) + (8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31;
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], p[r], o[d], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void weigh_odd(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d) {
+            f32x16 z;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float v = reinterpret_cast<const float*>(V)[(8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31 + 32 * d];
+                const bool bad = (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(bad ? 0.f : v, p[r], o[d], 0, 0, 0);
+                z = __builtin_amdgcn_mfma_f32_32x32x2f32(bad ? 1.f : 0.f, p[r], z, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = z[r] > 0.f ? __builtin_nanf("") : o[d][r];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __device__ static __forceinline__ bool not_finite(const f32x4& x) {
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bad |= (__float_as_uint(x[k]) & 0x7F800000u) == 0x7F800000u;
+        return bad;
+    }
+};
+
+// ROWS keys' K and V on their way from the pool to LDS, spread over NWS waves.  A request of a wave is 8 rows x 128 bytes;
+// request m of a tile covers rows 8 (m / (CH / 8)) and on, chunks 8 (m % (CH / 8)) and on: LDS addresses of one lane differ
+// by constants from request to request.
+template <typename T, int DH, int ROWS, int NWS>
+struct Stage {
+    typedef Prod<T, DH> P_;
+    static constexpr int N = ROWS * P_::CH / 64 / NWS, W = P_::CH / 8;
+    f32x4 k[N], v[N];
+    int r0, c0;
+    __device__ __forceinline__ Stage(int lane, int w) {
+        P_::piece(lane, r0, c0);
+        if constexpr (NWS > 1) {                  // wave w takes requests w N .. w N + N - 1
+            r0 += 8 * (w * N / W);
+            c0 += 8 * (w * N % W);
+        }
+    }
+    // (N is a multiple of W or the other way round, so a wave's requests are a rectangle)
+    __device__ __forceinline__ int row(int n) const { return r0 + 8 * (n / W); }
+    __device__ __forceinline__ int chunk(int n) const { return c0 + 8 * (n % W); }
+    // at: lane r's key_row of the tile's key r.  Rows that are nowhere read row 0 and are zeroed, so no load is masked.
+    __device__ __forceinline__ void load(const PagedArgs& a, unsigned at, bool whole) {
+        const unsigned bytes = a.dh * (unsigned)sizeof(T);
+        const unsigned safe = at == NONE ? 0u : at;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const unsigned ch = 16u * chunk(n);
+            const size_t off = (size_t)__shfl(safe, row(n), 64) * bytes + (whole || ch < bytes ? ch : 0u);
+            k[n] = *reinterpret_cast<const f32x4*>((const char*)a.kc + off);
+            v[n] = *reinterpret_cast<const f32x4*>((const char*)a.vc + off);
+        }
+    }
+    __device__ __forceinline__ void clean(const PagedArgs& a, unsigned at) {
+        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const bool keep = __shfl(at, row(n), 64) != NONE && 16 * chunk(n) < a.dh * (int)sizeof(T);
+            k[n] = keep ? k[n] : z;
+            v[n] = keep ? v[n] : z;
+        }
+    }
+    __device__ __forceinline__ bool v_not_finite() const {
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < N; ++n) bad |= P_::not_finite(v[n]);
+        return __any(bad);
+    }
+    __device__ __forceinline__ void store(char* K, char* V) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            *reinterpret_cast<f32x4*>(K + P_::koff(row(n), chunk(n))) = k[n];
+            *reinterpret_cast<f32x4*>(V + P_::voff(row(n), chunk(n))) = v[n];
+        }
+    }
+};
+
+// One wave's 32 rows, a row on each lane (and on lane ^ 32, which holds the other half of the keys of a tile).
+template <typename T, int DH>
+struct Rows {
+    typedef Prod<T, DH> P_;
+    typename P_::QFrag q[P_::NQ];
+    f32x16 o[DH / 32];
+    float m, l, c, bias;          // running maximum (raw scores), sum, scale * log2e, slope in raw-score units
+    int limit, at;                // last key this row sees, its position
+    int first_limit, last_limit;  // the smallest and largest limit of the wave's rows
+
+    // row: this lane's row of q (element pointer at its head), or NULL
+    __device__ __forceinline__ void begin(const PagedArgs& a, const T* row, int h5, float slope, int limit_, int at_) {
+        c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
+        bias = slope * LOG2E / c;
+        limit = limit_;
+        at = at_;
+        int lo = row ? limit_ : 0x7FFFFFFF, hi = row ? limit_ : -1;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) {
+            lo = min(lo, __shfl_xor(lo, s, 64));
+            hi = max(hi, __shfl_xor(hi, s, 64));
+        }
+        first_limit = __builtin_amdgcn_readfirstlane(lo);
+        last_limit = __builtin_amdgcn_readfirstlane(hi);
+        m = NEG;
+        l = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < P_::NQ; ++ks) {
+            const int ch = P_::qchunk(ks, h5);
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (row && ch * 16 < a.dh * (int)sizeof(T)) x = *reinterpret_cast<const f32x4*>((const char*)row + ch * 16);
+            if (a.scale < 0.f) {                         // the sign moves into q, exactly
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    x[k] = __uint_as_float(__float_as_uint(x[k]) ^ (sizeof(T) == 2 ? 0x80008000u : 0x80000000u));
+            }
+            __builtin_memcpy(&q[ks], &x, 16);
+        }
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    }
+    // NB blocks of 32 keys from j0 on; seen: the keys that are somewhere; odd: some V value is not finite
+    template <int NB>
+    __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned long long seen, bool odd,
+                                         bool alibi, int h5) {
+        f32x16 s[NB];
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[tb][r] = 0.f;
+        if (alibi) {
+            const float lb = bias * (float)(j0 + 4 * h5 - at);
+#pragma unroll
+            for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[tb][r] = lb + bias * (float)(32 * tb + (r & 3) + 8 * (r >> 2));
+        }
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb) s[tb] = pr.scores(K + tb * P_::KB, q, s[tb]);
+        const unsigned long long all = NB == 2 ? ~0ull : 0xFFFFFFFFull;
+        if (seen != all || j0 + 32 * NB - 1 > first_limit) {          // uniform
+            const int dj = limit - j0 - 4 * h5;
+            const unsigned long long mine = seen >> (4 * h5);
+#pragma unroll
+            for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int kk = 32 * tb + (r & 3) + 8 * (r >> 2);
+                    if (kk > dj || !((mine >> kk) & 1)) s[tb][r] = -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[tb][r]);
+        mx = half_swap_max(mx);
+        // the stale maximum stays while no row's grew by more than 2^8: weights are then at most 2^8, which fp32 sums and
+        // bf16 weights hold with the same relative precision
+        if (!__all((mx - m) * c <= RESCALE_LOG2)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = fast_exp2((m - mn) * c);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+        }
+        const float mc = m * c;
+        float sum = 0.f;
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[tb][r] = fast_exp2(fmaf(s[tb][r], c, -mc));
+                sum += s[tb][r];
+            }
+        l += sum;
+        if (!odd) {
+#pragma unroll
+            for (int tb = 0; tb < NB; ++tb) pr.weigh(V + tb * P_::VB, s[tb], o);
+        } else {
+            int nothing = 0;      // (keeps the compiler from reading the fragments of both branches ahead of them: 64 registers)
+            asm volatile("" : "+s"(nothing));
+#pragma unroll
+            for (int tb = 0; tb < NB; ++tb) {
+                pr.weigh_odd(V + tb * P_::VB + nothing, s[tb], o);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void put4(T* p, const float* x) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    } else {
+        bf16x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (bf16_t)x[k];
+        *reinterpret_cast<bf16x4*>(p) = v;
+    }
+}
+
+struct Item {
+    bool prefix, direct;         // prefix: rows of the whole batch; direct: the output itself, nothing to join
+    int b, hk, rt, rts, split;   // row tile and tiles in the grid; split: slot among the parts that are joined
+    int k0, k1, n, own;          // key range, rows of the sequence, own keys
+    long row0;                   // first row (of q) of the sequence
+};
+
+__device__ __forceinline__ bool own_item(const PagedArgs& a, int id, Item& it) {
+    it.prefix = false;
+    it.rts = a.rt_o;
+    it.split = id % a.So;
+    int rest = id / a.So;
+    it.hk = rest % a.Hkv;
+    rest /= a.Hkv;
+    it.rt = rest % a.rt_o;
+    it.b = rest / a.rt_o;
+    it.row0 = (long)it.b * a.R;
+    it.n = a.R;
+    if (a.cu) {                                   // (offsets that are none stay inside the rows)
+        it.row0 = min(max((long)a.cu[it.b], 0L), a.T);
+        it.n = (int)(min(max((long)a.cu[it.b + 1], it.row0), a.T) - it.row0);
+    }
+    it.own = min(max(a.lens[it.b], 0), a.width * a.page);
+    it.direct = !a.share && a.So == 1;
+    const int base = a.share ? a.P : 0, end = a.P + it.own;
+    // ranges of chunk_o keys, the last one open: it takes what a longer sequence than announced has left
+    it.k0 = base + it.split * a.chunk_o;
+    it.k1 = it.split == a.So - 1 ? end : min(end, it.k0 + a.chunk_o);
+    it.split += a.share ? a.Sp : 0;
+    return it.n > 0 && (it.k0 < it.k1 || it.split == (a.share ? a.Sp : 0));
+}
+__device__ __forceinline__ int own_parts(const PagedArgs& a, int own) {         // the own parts that exist, at least one
+    const int keys = a.share ? own : a.P + own;
+    return min(max((keys + a.chunk_o - 1) / a.chunk_o, 1), a.So);
+}
+__device__ __forceinline__ void prefix_item(const PagedArgs& a, int id, Item& it) {
+    // the row tiles of one (head, range) on one XCD (workgroup n runs on XCD n % 8), so that its L2 serves all but the first
+    const int pairs = a.Hkv * a.Sp, x = id & 7, rest = id >> 3;
+    it.prefix = true;
+    it.direct = false;
+    it.rts = a.rt_p;
+    it.rt = rest % a.rt_p;
+    const int pair = (rest / a.rt_p) * 8 + x;
+    it.hk = pair < pairs ? pair % a.Hkv : -1;
+    it.split = pair / a.Hkv;
+    it.b = 0;
+    it.row0 = 0;
+    it.n = (int)a.T;
+    it.own = 0;
+    it.k0 = it.split * a.chunk_p;
+    it.k1 = min(a.P, it.k0 + a.chunk_p);
+}
+
+// this lane's row of an item: its row of q (NULL: none), head, last key it sees, position
+template <typename T>
+__device__ __forceinline__ const T* item_row(const PagedArgs& a, const Item& it, long rho, int G, long& t, int& h, int& limit, int& at) {
+    t = it.row0 + rho / G;
+    h = it.hk * G + (int)(rho % G);
+    limit = at = a.P - 1;
+    if (rho >= (long)it.n * G || t >= a.T) return nullptr;
+    if (it.prefix) {
+        if (a.slopes) {
+            int b, r, n;
+            if (find_row(a, t, b, r, n)) at = a.P + a.lens[b] - n + r;
+        }
+    } else {
+        at = a.P + a.lens[it.b] - it.n + (int)(rho / G);
+        limit = max(at, a.P - 1);
+    }
+    return (const T*)a.q + t * a.qs + (long)h * a.dh;
+}
+
+template <typename T, int DH>
+__device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it, char* smem) {
+    typedef Prod<T, DH> P_;
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
+    const P_ pr(lane);
+    char* K = smem + w * (P_::KB + P_::VB);
+    char* V = K + P_::KB;
+    const int* own = a.table + (long)it.b * a.width;
+    for (int rt = it.rt; (long)rt * 32 < (long)it.n * G; rt += it.rts) {
+        long t;
+        int h, limit, at;
+        const T* row = item_row<T>(a, it, rt * 32L + l31, G, t, h, limit, at);
+        Rows<T, DH> rows;
+        rows.begin(a, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
+        const int end = min(it.k1, rows.last_limit + 1);
+        Stage<T, DH, 32, 1> st(lane, 0);
+        const bool whole = a.dh == DH;
+        int j = it.k0 + 32 * w;
+        unsigned kr = key_row(a, own, it.hk, j + l31, end), next = NONE;
+        if (j < end) {
+            st.load(a, kr, whole);
+            next = key_row(a, own, it.hk, j + 128 + l31, end);
+        }
+        while (j < end) {
+            const unsigned long long seen = __ballot(kr != NONE) & 0xFFFFFFFFull;
+            if (seen != 0xFFFFFFFFull || !whole) st.clean(a, kr);
+            const bool odd = j + 31 > rows.first_limit && st.v_not_finite();
+            st.store(K, V);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int j0 = j;
+            j += 128;
+            kr = next;
+            if (j < end) {
+                st.load(a, kr, whole);
+                next = key_row(a, own, it.hk, j + 128 + l31, end);
+            }
+            rows.template take<1>(pr, K, V, j0, seen, odd, a.slopes != nullptr, h5);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        // join the four waves: sums relative to each wave's maximum, through LDS (over the tiles)
+        constexpr int LD = DH + 4;
+        float* part = reinterpret_cast<float*>(smem);                   // [4][32][LD]
+        float* stat = part + 4 * 32 * LD;                               // [4][32][2]
+        const float lt = half_swap_sum(rows.l), m2 = rows.m * rows.c;
+        __syncthreads();
+        if (row) {
+            float* dst = part + (w * 32 + l31) * LD + 4 * h5;
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * g) =
+                        f32x4{rows.o[d][4 * g], rows.o[d][4 * g + 1], rows.o[d][4 * g + 2], rows.o[d][4 * g + 3]};
+            if (h5 == 0) {
+                stat[(w * 32 + l31) * 2] = m2;
+                stat[(w * 32 + l31) * 2 + 1] = lt;
+            }
+        }
+        __syncthreads();
+        const int nr = (int)min(32L, (long)it.n * G - rt * 32L), quads = a.dh / 4;
+        for (int e = tid; e < nr * quads; e += 256) {
+            const int rr = e / quads, d0 = 4 * (e - rr * quads);
+            const long rho = rt * 32L + rr, tt = it.row0 + rho / G;
+            if (tt >= a.T) continue;
+            float mm = stat[rr * 2], f[4], x[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+            for (int ww = 1; ww < 4; ++ww) mm = fmaxf(mm, stat[(ww * 32 + rr) * 2]);
+#pragma unroll
+            for (int ww = 0; ww < 4; ++ww) {
+                f[ww] = fast_exp2(stat[(ww * 32 + rr) * 2] - mm);
+                den = fmaf(stat[(ww * 32 + rr) * 2 + 1], f[ww], den);
+                const f32x4 p = *reinterpret_cast<const f32x4*>(part + (ww * 32 + rr) * LD + d0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = fmaf(p[k], f[ww], x[k]);
+            }
+            const long orow = tt * a.Hq + it.hk * G + rho % G;
+            if (it.direct) {
+                const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] *= inv;
+                put4((T*)a.out + orow * a.dh + d0, x);
+            } else {
+                const long slot = (long)it.split * a.T * a.Hq + orow;
+                put4(a.acc + slot * a.dh + d0, x);
+                if (d0 == 0) {
+                    a.ml[2 * slot] = mm;
+                    a.ml[2 * slot + 1] = den;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int DH>
+__device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, char* smem) {
+    typedef Prod<T, DH> P_;
+    constexpr int TB = 2 * (P_::KB + P_::VB);                           // one 64-key buffer: K, then V
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
+    const P_ pr(lane);
+    int* odd_tile = reinterpret_cast<int*>(smem + 2 * TB);              // [2]: 1 + the tile whose V is not finite
+    const int* own = a.table + (long)it.b * a.width;
+    for (int rt = it.rt; (long)rt * 128 < (long)it.n * G; rt += it.rts) {
+        long t;
+        int h, limit, at;
+        const T* row = item_row<T>(a, it, rt * 128L + 32 * w + l31, G, t, h, limit, at);
+        Rows<T, DH> rows;
+        rows.begin(a, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
+        // the range ends behind the last key any row of the workgroup sees; masked keys begin behind the first row's
+        int end = it.k1, sure = it.k1;
+        if (!it.prefix) {
+            const long lastr = min((long)it.n * G, rt * 128L + 128) - 1;
+            const int p0 = a.P + a.lens[it.b] - it.n;
+            end = min(end, max(p0 + (int)(lastr / G), a.P - 1) + 1);
+            sure = max(p0 + (int)(rt * 128L / G), a.P - 1) + 1;
+        }
+        const int ntiles = end > it.k0 ? (end - it.k0 + 63) / 64 : 0;
+        if (tid < 2) odd_tile[tid] = 0;
+        Stage<T, DH, 64, 4> st(lane, w);
+        const bool whole = a.dh == DH;
+        unsigned kr = NONE;
+        unsigned long long seen = 0, seen_next = 0;
+        // tiles are walked from the last one back (see attn_mfma.hip: with slopes the largest scores come first)
+        auto tile_of = [&](int n) { return it.k0 + (ntiles - 1 - n) * 64; };
+        auto fetch = [&](int n) {
+            kr = key_row(a, own, it.hk, tile_of(n) + lane, end);
+            st.load(a, kr, whole);
+        };
+        auto file = [&](int n) {
+            seen_next = __ballot(kr != NONE);
+            if (seen_next != ~0ull || !whole) st.clean(a, kr);
+            char* B = smem + (n & 1) * TB;
+            if (tile_of(n) + 63 >= sure && st.v_not_finite() && lane == 0) odd_tile[n & 1] = n + 1;
+            st.store(B, B + 2 * P_::KB);
+        };
+        __syncthreads();
+        if (ntiles > 0) {
+            fetch(0);
+            file(0);
+            seen = seen_next;
+            if (ntiles > 1) fetch(1);
+        }
+        __syncthreads();
+        for (int n = 0; n < ntiles; ++n) {
+            const int j0 = tile_of(n);
+            if (n + 1 < ntiles) file(n + 1);
+            if (n + 2 < ntiles) fetch(n + 2);
+            const char* B = smem + (n & 1) * TB;
+            if (j0 <= rows.last_limit)                                  // uniform in the wave
+                rows.template take<2>(pr, B, B + 2 * P_::KB, j0, seen, odd_tile[n & 1] == n + 1, a.slopes != nullptr, h5);
+            seen = seen_next;
+            __syncthreads();
+        }
+        const float lt = half_swap_sum(rows.l);
+        if (row) {
+            const long orow = t * a.Hq + h;
+            const long slot = (long)it.split * a.T * a.Hq + orow;
+            const float inv = it.direct ? (lt == 0.f ? 0.f : 1.f / lt) : 1.f;
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d0 = 32 * d + 8 * g + 4 * h5;
+                    if (d0 >= a.dh) continue;
+                    float x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = rows.o[d][4 * g + k] * inv;
+                    if (it.direct) put4((T*)a.out + orow * a.dh + d0, x);
+                    else put4(a.acc + slot * a.dh + d0, x);
+                }
+            if (!it.direct && h5 == 0) {
+                a.ml[2 * slot] = rows.m * rows.c;
+                a.ml[2 * slot + 1] = lt;
+            }
+        }
+    }
+}
+
+template <typename T, int DH>
+constexpr int attn_smem() {
+    typedef Prod<T, DH> P_;
+    const int priv = 4 * (P_::KB + P_::VB), join = 4 * 32 * (DH + 4) * 4 + 4 * 32 * 2 * 4, shared = 4 * (P_::KB + P_::VB) + 16;
+    return join > shared ? (join > priv ? join : priv) : (shared > priv ? shared : priv);
+}
+
+// BODY_P, BODY_O: 0 private, 1 shared, for prefix and own items
+template <typename T, int DH, int BODY_P, int BODY_O>
+__global__ __launch_bounds__(256, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char paged_smem[];
+    Item it;
+    int id = blockIdx.x;
+    if (id < a.n_items_p) {
+        prefix_item(a, id, it);
+        if (it.hk < 0) return;                                          // (whole workgroups, before any barrier)
+        if constexpr (BODY_P) shared_item<T, DH>(a, it, paged_smem);
+        else private_item<T, DH>(a, it, paged_smem);
+    } else {
+        if (!own_item(a, id - a.n_items_p, it)) return;
+        if constexpr (BODY_O) shared_item<T, DH>(a, it, paged_smem);
+        else private_item<T, DH>(a, it, paged_smem);
+    }
+}
+
+// rows of no sequence in a direct launch; every row in a joined one: lanes of 4 values, quads lanes a row
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
+    const int quads = a.dh / 4;
+    const long e = (long)blockIdx.x * 256 + threadIdx.x, row = e / quads;
+    if (row >= a.T * a.Hq) return;
+    const int d0 = 4 * (int)(e - row * quads);
+    int b, r, n;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool real = find_row(a, row / a.Hq, b, r, n);
+    const bool direct = !a.share && a.So == 1;
+    if (direct && real) return;
+    if (real) {
+        const int own = min(max(a.lens[b], 0), a.width * a.page), parts = (a.share ? a.Sp : 0) + own_parts(a, own);
+        const long step = a.T * a.Hq;
+        float mm = NEG, den = 0.f;
+        for (int s = 0; s < parts; ++s) {
+            const long slot = s * step + row;
+            const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
+            const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
+            const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
+            mm = mn;
+            den = den * f0 + l * f1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
+        }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] *= inv;
+    }
+    put4((T*)a.out + row * a.dh + d0, x);
+}
+
+// Heads wider than 128: one workgroup of 4 waves per (row, head); a key row is spread over lpr lanes, 16 bytes each.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, int lpr) {
     constexpr int N = 16 / sizeof(T);
@@ -109,11 +762,81 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, 
     }
 }
 
+// ---- the split: how rows and keys become work items -------------------------------------------------------------------
+struct Plan {
+    bool rows_only;                  // the row kernel
+    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, wide_p, wide_o;
+};
+
+inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
+Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int max_len, int dtype) {
+    Plan p = {};
+    p.rows_only = dh > 128;                            // a wave's sums, q and staged keys no longer fit its registers
+    const long G = Hq / Hkv, rows = (long)max_rows * G;
+    p.wide_o = rows > 32;
+    p.rt_o = (int)ceil_div(rows, p.wide_o ? 128 : 32);
+    // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
+    // sequence whose rows fill a tile by themselves has nothing to gain.
+    p.share = P > 0 && B > 1 && T * G < 128L * B;
+    constexpr long TARGET = 1024;                      // workgroups: two on each of 256 CUs, twice over
+    auto parts = [&](long base, long keys, int wide, int& chunk) {
+        const long least = wide ? 256 : 128;           // fewer keys than that an item spends its time on beginning and end
+        long s = ceil_div(TARGET, base);
+        if (s > ceil_div(keys, least)) s = ceil_div(keys, least);
+        if (s < 1) s = 1;
+        const long unit = wide ? 64 : 128;
+        chunk = (int)(ceil_div(ceil_div(keys, s), unit) * unit);
+        return (int)ceil_div(keys, chunk);
+    };
+    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.wide_o, p.chunk_o);
+    if (p.share) {
+        p.wide_p = T * G > 32;
+        p.rt_p = (int)ceil_div(T * G, p.wide_p ? 128 : 32);
+        p.Sp = parts((long)Hkv * p.rt_p, P, p.wide_p, p.chunk_p);
+    }
+    return p;
+}
+
+template <typename T, int DH, int BODY_P, int BODY_O>
+int launch_items(const PagedArgs& a, long items, hipStream_t st) {
+    constexpr int smem = attn_smem<T, DH>();
+    if (smem > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY_P, BODY_O>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+        MGX_REQUIRE(e == hipSuccess, MGX_ELAUNCH, "mgx_paged_attn: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O>), dim3((unsigned)items), dim3(256), smem, st, a);
+    MGX_CHECK_LAUNCH("paged_attn");
+    return MGX_OK;
+}
+
+template <typename T, int DH>
+int launch_paged(const PagedArgs& a, const Plan& p, long items, hipStream_t st) {
+    MGX_REQUIRE(items < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
+    // (own rows past 32 make the batch's rows past 32, so shared own items never meet private prefix items)
+    const int rc = p.wide_o   ? launch_items<T, DH, 1, 1>(a, items, st)
+                   : p.wide_p ? launch_items<T, DH, 1, 0>(a, items, st)
+                              : launch_items<T, DH, 0, 0>(a, items, st);
+    if (rc) return rc;
+    // (ragged rows in a direct launch: the join kernel clears the rows of no sequence)
+    if (a.share || a.So > 1 || a.cu) {
+        const long blocks = ceil_div(a.T * a.Hq * (a.dh / 4), 256);
+        MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
+        hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+        MGX_CHECK_LAUNCH("paged_join");
+    }
+    return MGX_OK;
+}
+
 }  // namespace
 
 extern "C" long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows,
                                                 int max_len, int dtype) {
-    return 0;
+    if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || dh <= 0 || max_rows <= 0 || max_len <= 0 || prefix_len < 0) return 0;
+    const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
+    if (p.rows_only || (!p.share && p.So == 1)) return 0;
+    return (p.So + p.Sp) * T * Hq * (dh + 2L);
 }
 
 extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const void* vcache, const int* table,
@@ -136,13 +859,32 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
     MGX_REQUIRE((((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0, MGX_EINVAL,
                 "mgx_paged_attn: tensors must be 16-byte aligned");
     MGX_REQUIRE(Hq <= 65535, MGX_EUNSUPPORTED, "mgx_paged_attn: Hq=%d", Hq);
-    const PagedArgs a{q, kcache, vcache, out, table, lens, cu_rows, prefix, slopes, B, R, Hq, Hkv, dh, page, n_pages, width,
-                      prefix_len, max_rows, max_len, T, q_row_stride, scale};
-    int lpr = 1;
-    while (lpr * N < dh) lpr *= 2;
-    const dim3 grid((unsigned)T, Hq);
-    if (dtype == MGX_F32) hipLaunchKernelGGL((paged_attn_row_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, a, lpr);
-    else hipLaunchKernelGGL((paged_attn_row_kernel<bf16_t>), grid, dim3(256), 0, (hipStream_t)stream, a, lpr);
-    MGX_CHECK_LAUNCH("paged_attn");
-    return MGX_OK;
+    const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
+    MGX_REQUIRE(workspace || p.rows_only || (!p.share && p.So == 1), MGX_EINVAL, "mgx_paged_attn: no workspace");
+    MGX_REQUIRE((long)n_pages * Hkv * page < 0xFFFFFFFFL, MGX_EUNSUPPORTED, "mgx_paged_attn: pool of more than 2^32 rows");
+    PagedArgs a = {};
+    a.q = q, a.kc = kcache, a.vc = vcache, a.out = out;
+    a.table = table, a.lens = lens, a.cu = cu_rows, a.prefix = prefix, a.slopes = slopes;
+    a.B = B, a.R = R, a.Hq = Hq, a.Hkv = Hkv, a.dh = dh, a.page = page, a.n_pages = n_pages, a.width = width, a.P = prefix_len;
+    a.shift = (page & (page - 1)) ? -1 : __builtin_ctz(page);
+    a.T = T, a.qs = q_row_stride, a.scale = scale;
+    a.share = p.share, a.Sp = p.Sp, a.So = p.So, a.chunk_p = p.chunk_p, a.chunk_o = p.chunk_o;
+    a.rt_p = p.rt_p, a.rt_o = p.rt_o;
+    hipStream_t st = (hipStream_t)stream;
+    if (p.rows_only) {
+        const dim3 grid((unsigned)T, Hq);
+        int lpr = 1;
+        while (lpr * N < dh) lpr *= 2;
+        if (dtype == MGX_F32) hipLaunchKernelGGL((paged_attn_row_kernel<float>), grid, dim3(256), 0, st, a, lpr);
+        else hipLaunchKernelGGL((paged_attn_row_kernel<bf16_t>), grid, dim3(256), 0, st, a, lpr);
+        MGX_CHECK_LAUNCH("paged_attn_row");
+        return MGX_OK;
+    }
+    a.acc = workspace;
+    a.ml = workspace + (p.So + p.Sp) * T * Hq * (long)dh;
+    a.n_items_p = p.share ? (int)(ceil_div((long)Hkv * p.Sp, 8) * 8 * p.rt_p) : 0;
+    MGX_REQUIRE(!p.share || ceil_div((long)Hkv * p.Sp, 8) * 8 * p.rt_p < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
+    const long items = a.n_items_p + (long)B * Hkv * p.rt_o * p.So;
+    if (dtype == MGX_F32) return dh <= 64 ? launch_paged<float, 64>(a, p, items, st) : launch_paged<float, 128>(a, p, items, st);
+    return dh <= 64 ? launch_paged<bf16_t, 64>(a, p, items, st) : launch_paged<bf16_t, 128>(a, p, items, st);
 }
