@@ -10,12 +10,12 @@
 // that read one K/V head - the G = Hq / Hkv query heads of a group are rows of the same tile - against a range of keys.
 //   own items     rows of one sequence, its own keys (all keys, where the prefix is not taken apart)
 //   prefix items  rows of the WHOLE batch, prefix keys: K and V of the prefix are read once per row tile of the batch
-// Every product is arranged as K . Q^T and V^T . P^T on 32x32 MFMA tiles: the row (query) is on the lane, so a row's
-// maximum and sum need one exchange between half-waves per tile, and P goes from the first product's accumulators to the
-// second's operand without leaving the registers.  Two bodies in one launch:
-//   private  <= 32 rows: memory bound.  The four waves take alternate 32-key tiles, each through LDS of its own with the
-//            next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
-//   shared   <= 128 rows, 32 a wave: 64-key tiles in LDS, double buffered, shared by the four waves.
+// Every product is arranged as K . Q^T and V^T . P^T on MFMA tiles: the row (query) is on the lane, so a row's maximum and
+// sum need one or two exchanges between lanes per tile, and P goes from the first product's accumulators to the second's
+// operand without leaving the registers (the order of the keys in it is free, V is read in the same one).  Two bodies:
+//   private  <= 16 or 32 rows (16x16 tiles): memory bound.  The waves take alternate 32-key tiles, each through LDS of its
+//            own with the next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
+//   shared   32 rows a wave (32x32 tiles): 64-key tiles in LDS, double buffered, shared by the workgroup.
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
 #include "attn_mfma_common.h"
 
@@ -197,12 +197,162 @@ template <int DH> struct Prod<float, DH> {        // v_mfma_f32_32x32x2_f32: the
     }
 };
 
+// ---- 16x16 tiles: RT x 16 rows a wave, 32 keys at a time ----------------------------------------------------------------
+template <typename T, int DH> struct Prod16;
+
+template <int DH> struct Prod16<bf16_t, DH> {     // v_mfma_f32_16x16x32_bf16
+    static constexpr int CH = DH / 8, G8 = 8 * DH * 2;
+    static constexpr int KB = 32 * DH * 2, VB = KB;
+    typedef bf16x8 QFrag;
+    static constexpr int NQ = DH / 32;
+    int k0, v0;
+    // 8-row x 32-column sub-tiles of 512 bytes; the XOR spreads the four rows of equal row & 3 over a 64-byte line (row
+    // reads of 16 rows) and puts rows 0-3 and 4-7 on different 32-byte halves (transposed reads): both conflict-free
+    __device__ static __forceinline__ int swap(int row) { return 2 * ((row >> 2) & 1) | ((row >> 3) & 1); }
+    __device__ static __forceinline__ int koff(int row, int ch) {
+        return G8 * (row >> 3) + 512 * (ch >> 2) + 64 * (row & 7) + 16 * ((ch & 3) ^ swap(row));
+    }
+    __device__ static __forceinline__ int voff(int row, int ch) { return koff(row, ch); }
+    __device__ static __forceinline__ void piece(int lane, int& row, int& ch) { Prod<bf16_t, DH>::piece(lane, row, ch); }
+    __device__ static __forceinline__ bool not_finite(const f32x4& x) { return Prod<bf16_t, DH>::not_finite(x); }
+    __device__ __forceinline__ Prod16(int lane) {
+        const int l15 = lane & 15, g = lane >> 4, q = l15 >> 2, p = l15 & 3;
+        k0 = koff(l15, g);
+        v0 = koff(4 * g + q, p >> 1) + 8 * (p & 1);
+    }
+    __device__ static __forceinline__ int qchunk(int ks, int g) { return 4 * ks + g; }
+    // keys 16 kt + .. against the rows of q
+    template <int RT>
+    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[RT][NQ], f32x4 (&s)[RT][2]) const {
+#pragma unroll
+        for (int ks = 0; ks < NQ; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const bf16x8 k = lds_read16(K + k0 + 2 * G8 * kt + 512 * ks);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[rt][ks], s[rt][kt], 0, 0, 0);
+            }
+    }
+    __device__ static __forceinline__ bf16x8 pack(const f32x4 (&p)[2]) {
+        bf16x8 r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = (bf16_t)p[0][k], r[4 + k] = (bf16_t)p[1][k];
+        return r;
+    }
+    __device__ __forceinline__ bf16x8 vfrag(const char* V, int d) const {
+        const char* at = V + (v0 ^ (32 * (d & 1))) + 512 * (d >> 1);
+        return lds_read_tr_pair(at, at + 2 * G8);
+    }
+    // P is rounded to bf16 for the product (2^-8 relative each, signs independent); its sum is taken before that
+    template <int RT>
+    __device__ __forceinline__ void weigh(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
+        bf16x8 pf[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) pf[rt] = pack(p[rt]);
+#pragma unroll
+        for (int d = 0; d < DH / 16; ++d) {
+            const bf16x8 v = vfrag(V, d);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[rt], o[rt][d], 0, 0, 0);
+        }
+    }
+    // as Prod::weigh_odd
+    template <int RT>
+    __device__ __forceinline__ void weigh_odd(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
+#pragma unroll
+        for (int d = 0; d < DH / 16; ++d) {
+            bf16x8 v = vfrag(V, d), at;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bf16_t x = v[k];                 // (bit_cast of a vector-element lvalue reads element 0)
+                const bool bad = (__builtin_bit_cast(unsigned short, x) & 0x7F80) == 0x7F80;
+                at[k] = (bf16_t)(bad ? 1.f : 0.f);
+                v[k] = bad ? (bf16_t)0.f : x;
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const bf16x8 pf = pack(p[rt]);
+                const f32x4 z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at, pf, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf, o[rt][d], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[rt][d][r] = z[r] > 0.f ? __builtin_nanf("") : o[rt][d][r];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
+
+template <int DH> struct Prod16<float, DH> {      // v_mfma_f32_16x16x4_f32
+    static constexpr int CH = DH / 4;
+    static constexpr int VS = DH + 4;             // V row stride: the four rows a request reads, 4 apart, lie 16 banks apart
+    static constexpr int KB = 32 * DH * 4, VB = 32 * VS * 4;
+    typedef f32x4 QFrag;
+    static constexpr int NQ = DH / 16;
+    const int l15, g;
+    __device__ __forceinline__ Prod16(int lane) : l15(lane & 15), g(lane >> 4) {}
+    __device__ static __forceinline__ int koff(int row, int ch) { return row * DH * 4 + 16 * (ch ^ (row & 15)); }
+    __device__ static __forceinline__ int voff(int row, int ch) { return row * VS * 4 + 16 * ch; }
+    __device__ static __forceinline__ void piece(int lane, int& row, int& ch) { row = lane >> 3, ch = lane & 7; }
+    __device__ static __forceinline__ bool not_finite(const f32x4& x) { return Prod<float, DH>::not_finite(x); }
+    __device__ static __forceinline__ int qchunk(int ks, int g_) { return 4 * ks + g_; }
+    template <int RT>
+    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[RT][NQ], f32x4 (&s)[RT][2]) const {
+#pragma unroll
+        for (int c = 0; c < NQ; ++c)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const f32x4 k = *reinterpret_cast<const f32x4*>(K + koff(16 * kt + l15, 4 * c + g));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[rt][c][e], s[rt][kt], 0, 0, 0);
+            }
+    }
+    __device__ __forceinline__ float value(const char* V, int kt, int r, int d) const {
+        return reinterpret_cast<const float*>(V)[(16 * kt + 4 * g + r) * VS + l15 + 16 * d];
+    }
+    template <int RT>
+    __device__ __forceinline__ void weigh(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int d = 0; d < DH / 16; ++d) {
+                    const float v = value(V, kt, r, d);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[rt][kt][r], o[rt][d], 0, 0, 0);
+                }
+    }
+    template <int RT>
+    __device__ __forceinline__ void weigh_odd(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
+#pragma unroll
+        for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = value(V, kt, r, d);
+                        const bool bad = (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 0.f : v, p[rt][kt][r], o[rt][d], 0, 0, 0);
+                        z = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 1.f : 0.f, p[rt][kt][r], z, 0, 0, 0);
+                    }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[rt][d][r] = z[r] > 0.f ? __builtin_nanf("") : o[rt][d][r];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+};
+
 // ROWS keys' K and V on their way from the pool to LDS, spread over NWS waves.  A request of a wave is 8 rows x 128 bytes;
 // request m of a tile covers rows 8 (m / (CH / 8)) and on, chunks 8 (m % (CH / 8)) and on: LDS addresses of one lane differ
 // by constants from request to request.
-template <typename T, int DH, int ROWS, int NWS>
+template <typename P_, typename T, int DH, int ROWS, int NWS>
 struct Stage {
-    typedef Prod<T, DH> P_;
     static constexpr int N = ROWS * P_::CH / 64 / NWS, W = P_::CH / 8;
     f32x4 k[N], v[N];
     int r0, c0;
@@ -252,6 +402,19 @@ struct Stage {
     }
 };
 
+template <typename T, typename QFrag>
+__device__ __forceinline__ QFrag load_q(const PagedArgs& a, const T* row, int ch) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (row && ch * 16 < a.dh * (int)sizeof(T)) x = *reinterpret_cast<const f32x4*>((const char*)row + ch * 16);
+    if (a.scale < 0.f) {                                 // the scale's sign moves into q, exactly
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(__float_as_uint(x[k]) ^ (sizeof(T) == 2 ? 0x80008000u : 0x80000000u));
+    }
+    QFrag q;
+    __builtin_memcpy(&q, &x, 16);
+    return q;
+}
+
 // One wave's 32 rows, a row on each lane (and on lane ^ 32, which holds the other half of the keys of a tile).
 template <typename T, int DH>
 struct Rows {
@@ -279,17 +442,7 @@ struct Rows {
         m = NEG;
         l = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < P_::NQ; ++ks) {
-            const int ch = P_::qchunk(ks, h5);
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            if (row && ch * 16 < a.dh * (int)sizeof(T)) x = *reinterpret_cast<const f32x4*>((const char*)row + ch * 16);
-            if (a.scale < 0.f) {                         // the sign moves into q, exactly
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    x[k] = __uint_as_float(__float_as_uint(x[k]) ^ (sizeof(T) == 2 ? 0x80008000u : 0x80000000u));
-            }
-            __builtin_memcpy(&q[ks], &x, 16);
-        }
+        for (int ks = 0; ks < P_::NQ; ++ks) q[ks] = load_q<T, typename P_::QFrag>(a, row, P_::qchunk(ks, h5));
 #pragma unroll
         for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
@@ -365,6 +518,118 @@ struct Rows {
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+    }
+};
+
+// over the four 16-lane groups, each of which holds other keys of the same 16 rows
+__device__ __forceinline__ float quarter_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_swap_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// RT x 16 rows of a wave: row 16 rt + (lane & 15) on four lanes.
+template <typename T, int DH, int RT>
+struct Rows16 {
+    typedef Prod16<T, DH> P_;
+    typename P_::QFrag q[RT][P_::NQ];
+    f32x4 o[RT][DH / 16];
+    float m[RT], l[RT], bias[RT], c;
+    int limit[RT], at[RT], first_limit, last_limit;
+
+    __device__ __forceinline__ void begin(const PagedArgs& a) {
+        c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
+        first_limit = 0x7FFFFFFF;
+        last_limit = -1;
+    }
+    __device__ __forceinline__ void begin_row(const PagedArgs& a, int rt, const T* row, int g, float slope, int limit_, int at_) {
+        bias[rt] = slope * LOG2E / c;
+        limit[rt] = limit_;
+        at[rt] = at_;
+        int lo = row ? limit_ : 0x7FFFFFFF, hi = row ? limit_ : -1;
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) {
+            lo = min(lo, __shfl_xor(lo, s, 64));
+            hi = max(hi, __shfl_xor(hi, s, 64));
+        }
+        first_limit = min(first_limit, __builtin_amdgcn_readfirstlane(lo));
+        last_limit = max(last_limit, __builtin_amdgcn_readfirstlane(hi));
+        m[rt] = NEG;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < P_::NQ; ++ks) q[rt][ks] = load_q<T, typename P_::QFrag>(a, row, P_::qchunk(ks, g));
+#pragma unroll
+        for (int d = 0; d < DH / 16; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // 32 keys from j0 on (see Rows::take)
+    __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned seen, bool odd, bool alibi,
+                                         int g) {
+        f32x4 s[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (alibi) {
+                    const float lb = bias[rt] * (float)(j0 + 4 * g - at[rt]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[rt][kt][r] = lb + bias[rt] * (float)(16 * kt + r);
+                }
+            }
+        pr.template scores<RT>(K, q, s);
+        const bool mask = seen != 0xFFFFFFFFu || j0 + 31 > first_limit;          // uniform
+        bool grown = false;
+        float mx[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (mask) {
+                const int dj = limit[rt] - j0 - 4 * g;
+                const unsigned mine = seen >> (4 * g);
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * kt + r > dj || !((mine >> (16 * kt + r)) & 1)) s[rt][kt][r] = -INFINITY;
+            }
+            float x = s[rt][0][0];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x = fmaxf(x, s[rt][kt][r]);
+            mx[rt] = quarter_max(x);
+            grown |= !((mx[rt] - m[rt]) * c <= RESCALE_LOG2);
+        }
+        if (__any(grown)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float mn = fmaxf(m[rt], mx[rt]);
+                const float alpha = fast_exp2((m[rt] - mn) * c);
+                m[rt] = mn;
+                l[rt] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[rt][d][r] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const float mc = m[rt] * c;
+            float sum = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[rt][kt][r] = fast_exp2(fmaf(s[rt][kt][r], c, -mc));
+                    sum += s[rt][kt][r];
+                }
+            l[rt] += sum;
+        }
+        if (!odd) pr.template weigh<RT>(V, s, o);
+        else pr.template weigh_odd<RT>(V, s, o);
     }
 };
 
@@ -452,83 +717,89 @@ __device__ __forceinline__ const T* item_row(const PagedArgs& a, const Item& it,
     return (const T*)a.q + t * a.qs + (long)h * a.dh;
 }
 
-template <typename T, int DH>
+template <typename T, int DH, int RT, int NW>
 __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it, char* smem) {
-    typedef Prod<T, DH> P_;
-    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
+    typedef Prod16<T, DH> P_;
+    constexpr int TR = 16 * RT, STEP = 32 * NW;
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, l31 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
     const P_ pr(lane);
     char* K = smem + w * (P_::KB + P_::VB);
     char* V = K + P_::KB;
     const int* own = a.table + (long)it.b * a.width;
-    for (int rt = it.rt; (long)rt * 32 < (long)it.n * G; rt += it.rts) {
-        long t;
-        int h, limit, at;
-        const T* row = item_row<T>(a, it, rt * 32L + l31, G, t, h, limit, at);
-        Rows<T, DH> rows;
-        rows.begin(a, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
+    for (int rt = it.rt; (long)rt * TR < (long)it.n * G; rt += it.rts) {
+        Rows16<T, DH, RT> rows;
+        rows.begin(a);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            long t;
+            int h, limit, at;
+            const T* row = item_row<T>(a, it, rt * (long)TR + 16 * i + l15, G, t, h, limit, at);
+            rows.begin_row(a, i, row, g, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
+        }
         const int end = min(it.k1, rows.last_limit + 1);
-        Stage<T, DH, 32, 1> st(lane, 0);
         const bool whole = a.dh == DH;
+        Stage<P_, T, DH, 32, 1> st(lane, 0);
         int j = it.k0 + 32 * w;
         unsigned kr = key_row(a, own, it.hk, j + l31, end), next = NONE;
         if (j < end) {
             st.load(a, kr, whole);
-            next = key_row(a, own, it.hk, j + 128 + l31, end);
+            next = key_row(a, own, it.hk, j + STEP + l31, end);
         }
         while (j < end) {
-            const unsigned long long seen = __ballot(kr != NONE) & 0xFFFFFFFFull;
-            if (seen != 0xFFFFFFFFull || !whole) st.clean(a, kr);
+            const unsigned seen = (unsigned)__ballot(kr != NONE);
+            if (seen != 0xFFFFFFFFu || !whole) st.clean(a, kr);
             const bool odd = j + 31 > rows.first_limit && st.v_not_finite();
             st.store(K, V);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             const int j0 = j;
-            j += 128;
+            j += STEP;
             kr = next;
             if (j < end) {
                 st.load(a, kr, whole);
-                next = key_row(a, own, it.hk, j + 128 + l31, end);
+                next = key_row(a, own, it.hk, j + STEP + l31, end);
             }
-            rows.template take<1>(pr, K, V, j0, seen, odd, a.slopes != nullptr, h5);
+            rows.take(pr, K, V, j0, seen, odd, a.slopes != nullptr, g);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
-        // join the four waves: sums relative to each wave's maximum, through LDS (over the tiles)
+        // join the waves: sums relative to each wave's maximum, through LDS (over the tiles)
         constexpr int LD = DH + 4;
-        float* part = reinterpret_cast<float*>(smem);                   // [4][32][LD]
-        float* stat = part + 4 * 32 * LD;                               // [4][32][2]
-        const float lt = half_swap_sum(rows.l), m2 = rows.m * rows.c;
+        float* part = reinterpret_cast<float*>(smem);                   // [NW][TR][LD]
+        float* stat = part + NW * TR * LD;                              // [NW][TR][2]
+        const int nr = (int)min((long)TR, (long)it.n * G - rt * (long)TR);
         __syncthreads();
-        if (row) {
-            float* dst = part + (w * 32 + l31) * LD + 4 * h5;
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d)
+        for (int i = 0; i < RT; ++i) {
+            const int r = 16 * i + l15;
+            const float lt = quarter_sum(rows.l[i]);
+            if (r < nr) {
+                float* dst = part + (w * TR + r) * LD + 4 * g;
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * g) =
-                        f32x4{rows.o[d][4 * g], rows.o[d][4 * g + 1], rows.o[d][4 * g + 2], rows.o[d][4 * g + 3]};
-            if (h5 == 0) {
-                stat[(w * 32 + l31) * 2] = m2;
-                stat[(w * 32 + l31) * 2 + 1] = lt;
+                for (int d = 0; d < DH / 16; ++d) *reinterpret_cast<f32x4*>(dst + 16 * d) = rows.o[i][d];
+                if (g == 0) {
+                    stat[(w * TR + r) * 2] = rows.m[i] * rows.c;
+                    stat[(w * TR + r) * 2 + 1] = lt;
+                }
             }
         }
         __syncthreads();
-        const int nr = (int)min(32L, (long)it.n * G - rt * 32L), quads = a.dh / 4;
-        for (int e = tid; e < nr * quads; e += 256) {
+        const int quads = a.dh / 4;
+        for (int e = tid; e < nr * quads; e += 64 * NW) {
             const int rr = e / quads, d0 = 4 * (e - rr * quads);
-            const long rho = rt * 32L + rr, tt = it.row0 + rho / G;
+            const long rho = rt * (long)TR + rr, tt = it.row0 + rho / G;
             if (tt >= a.T) continue;
-            float mm = stat[rr * 2], f[4], x[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+            float mm = stat[rr * 2], x[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
 #pragma unroll
-            for (int ww = 1; ww < 4; ++ww) mm = fmaxf(mm, stat[(ww * 32 + rr) * 2]);
+            for (int ww = 1; ww < NW; ++ww) mm = fmaxf(mm, stat[(ww * TR + rr) * 2]);
 #pragma unroll
-            for (int ww = 0; ww < 4; ++ww) {
-                f[ww] = fast_exp2(stat[(ww * 32 + rr) * 2] - mm);
-                den = fmaf(stat[(ww * 32 + rr) * 2 + 1], f[ww], den);
-                const f32x4 p = *reinterpret_cast<const f32x4*>(part + (ww * 32 + rr) * LD + d0);
+            for (int ww = 0; ww < NW; ++ww) {
+                const float f = fast_exp2(stat[(ww * TR + rr) * 2] - mm);
+                den = fmaf(stat[(ww * TR + rr) * 2 + 1], f, den);
+                const f32x4 p = *reinterpret_cast<const f32x4*>(part + (ww * TR + rr) * LD + d0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = fmaf(p[k], f[ww], x[k]);
+                for (int k = 0; k < 4; ++k) x[k] = fmaf(p[k], f, x[k]);
             }
             const long orow = tt * a.Hq + it.hk * G + rho % G;
             if (it.direct) {
@@ -549,32 +820,33 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
     }
 }
 
-template <typename T, int DH>
+template <typename T, int DH, int NW>
 __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod<T, DH> P_;
     constexpr int TB = 2 * (P_::KB + P_::VB);                           // one 64-key buffer: K, then V
+    constexpr long TR = 32 * NW;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
     const P_ pr(lane);
     int* odd_tile = reinterpret_cast<int*>(smem + 2 * TB);              // [2]: 1 + the tile whose V is not finite
     const int* own = a.table + (long)it.b * a.width;
-    for (int rt = it.rt; (long)rt * 128 < (long)it.n * G; rt += it.rts) {
+    for (int rt = it.rt; rt * TR < (long)it.n * G; rt += it.rts) {
         long t;
         int h, limit, at;
-        const T* row = item_row<T>(a, it, rt * 128L + 32 * w + l31, G, t, h, limit, at);
+        const T* row = item_row<T>(a, it, rt * TR + 32 * w + l31, G, t, h, limit, at);
         Rows<T, DH> rows;
         rows.begin(a, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
         // the range ends behind the last key any row of the workgroup sees; masked keys begin behind the first row's
         int end = it.k1, sure = it.k1;
         if (!it.prefix) {
-            const long lastr = min((long)it.n * G, rt * 128L + 128) - 1;
+            const long lastr = min((long)it.n * G, rt * TR + TR) - 1;
             const int p0 = a.P + a.lens[it.b] - it.n;
             end = min(end, max(p0 + (int)(lastr / G), a.P - 1) + 1);
-            sure = max(p0 + (int)(rt * 128L / G), a.P - 1) + 1;
+            sure = max(p0 + (int)(rt * TR / G), a.P - 1) + 1;
         }
         const int ntiles = end > it.k0 ? (end - it.k0 + 63) / 64 : 0;
         if (tid < 2) odd_tile[tid] = 0;
-        Stage<T, DH, 64, 4> st(lane, w);
+        Stage<P_, T, DH, 64, NW> st(lane, w);
         const bool whole = a.dh == DH;
         unsigned kr = NONE;
         unsigned long long seen = 0, seen_next = 0;
@@ -634,28 +906,31 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
     }
 }
 
-template <typename T, int DH>
-constexpr int attn_smem() {
-    typedef Prod<T, DH> P_;
-    const int priv = 4 * (P_::KB + P_::VB), join = 4 * 32 * (DH + 4) * 4 + 4 * 32 * 2 * 4, shared = 4 * (P_::KB + P_::VB) + 16;
-    return join > shared ? (join > priv ? join : priv) : (shared > priv ? shared : priv);
+// BODY: 0 / 1 private with 16 / 32 rows, 2 shared
+template <typename T, int DH, int BODY, int NW>
+constexpr int body_smem() {
+    if (BODY == 2) return 4 * (Prod<T, DH>::KB + Prod<T, DH>::VB) + 16;
+    const int tiles = NW * (Prod16<T, DH>::KB + Prod16<T, DH>::VB), rows = BODY == 1 ? 32 : 16, join = NW * rows * (DH + 4 + 2) * 4;
+    return tiles > join ? tiles : join;
+}
+template <typename T, int DH, int BODY, int NW>
+__device__ __forceinline__ void body(const PagedArgs& a, const Item& it, char* smem) {
+    if constexpr (BODY == 2) shared_item<T, DH, NW>(a, it, smem);
+    else private_item<T, DH, BODY + 1, NW>(a, it, smem);
 }
 
-// BODY_P, BODY_O: 0 private, 1 shared, for prefix and own items
-template <typename T, int DH, int BODY_P, int BODY_O>
-__global__ __launch_bounds__(256, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a) {
+template <typename T, int DH, int BODY_P, int BODY_O, int NW>
+__global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a) {
     extern __shared__ __attribute__((aligned(16))) char paged_smem[];
     Item it;
-    int id = blockIdx.x;
+    const int id = blockIdx.x;
     if (id < a.n_items_p) {
         prefix_item(a, id, it);
         if (it.hk < 0) return;                                          // (whole workgroups, before any barrier)
-        if constexpr (BODY_P) shared_item<T, DH>(a, it, paged_smem);
-        else private_item<T, DH>(a, it, paged_smem);
+        body<T, DH, BODY_P, NW>(a, it, paged_smem);
     } else {
         if (!own_item(a, id - a.n_items_p, it)) return;
-        if constexpr (BODY_O) shared_item<T, DH>(a, it, paged_smem);
-        else private_item<T, DH>(a, it, paged_smem);
+        body<T, DH, BODY_O, NW>(a, it, paged_smem);
     }
 }
 
@@ -765,7 +1040,7 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, 
 // ---- the split: how rows and keys become work items -------------------------------------------------------------------
 struct Plan {
     bool rows_only;                  // the row kernel
-    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, wide_p, wide_o;
+    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, body_p, body_o, nw;
 };
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
@@ -774,50 +1049,58 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     Plan p = {};
     p.rows_only = dh > 128;                            // a wave's sums, q and staged keys no longer fit its registers
     const long G = Hq / Hkv, rows = (long)max_rows * G;
-    p.wide_o = rows > 32;
-    p.rt_o = (int)ceil_div(rows, p.wide_o ? 128 : 32);
+    auto body_of = [](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : 2; };
+    p.body_o = body_of(rows);
     // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
     // sequence whose rows fill a tile by themselves has nothing to gain.
     p.share = P > 0 && B > 1 && T * G < 128L * B;
+    p.body_p = p.share ? body_of(T * G) : p.body_o;
+    if (p.body_p == 1) p.body_o = 1;                   // (one instance fewer: private items of 32 rows take 16, too)
+    if (p.body_o == 2) p.body_p = 2;
+    // shared items: eight waves (256 rows), four where fp32 tiles of dh 128 would pass the LDS
+    p.nw = p.body_p == 2 && !(dtype == MGX_F32 && dh > 64) ? 8 : 4;
     constexpr long TARGET = 1024;                      // workgroups: two on each of 256 CUs, twice over
-    auto parts = [&](long base, long keys, int wide, int& chunk) {
-        const long least = wide ? 256 : 128;           // fewer keys than that an item spends its time on beginning and end
+    auto tile_rows = [&](int body) { return body == 2 ? 32L * p.nw : 16L * (body + 1); };
+    auto parts = [&](long base, long keys, int body, int& chunk) {
+        const long unit = body == 2 ? 64 : 32 * p.nw, least = 256;      // fewer keys are all beginning and end
         long s = ceil_div(TARGET, base);
         if (s > ceil_div(keys, least)) s = ceil_div(keys, least);
         if (s < 1) s = 1;
-        const long unit = wide ? 64 : 128;
         chunk = (int)(ceil_div(ceil_div(keys, s), unit) * unit);
         return (int)ceil_div(keys, chunk);
     };
-    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.wide_o, p.chunk_o);
+    p.rt_o = (int)ceil_div(rows, tile_rows(p.body_o));
+    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, p.chunk_o);
     if (p.share) {
-        p.wide_p = T * G > 32;
-        p.rt_p = (int)ceil_div(T * G, p.wide_p ? 128 : 32);
-        p.Sp = parts((long)Hkv * p.rt_p, P, p.wide_p, p.chunk_p);
+        p.rt_p = (int)ceil_div(T * G, tile_rows(p.body_p));
+        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, p.chunk_p);
     }
     return p;
 }
 
-template <typename T, int DH, int BODY_P, int BODY_O>
+template <typename T, int DH, int BODY_P, int BODY_O, int NW>
 int launch_items(const PagedArgs& a, long items, hipStream_t st) {
-    constexpr int smem = attn_smem<T, DH>();
+    constexpr int sp = body_smem<T, DH, BODY_P, NW>(), so = body_smem<T, DH, BODY_O, NW>(), smem = sp > so ? sp : so;
+    static_assert(smem <= 160 * 1024, "LDS of a CU");
     if (smem > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY_P, BODY_O>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY_P, BODY_O, NW>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, smem);
         MGX_REQUIRE(e == hipSuccess, MGX_ELAUNCH, "mgx_paged_attn: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O>), dim3((unsigned)items), dim3(256), smem, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O, NW>), dim3((unsigned)items), dim3(64 * NW), smem, st, a);
     MGX_CHECK_LAUNCH("paged_attn");
     return MGX_OK;
 }
 
 template <typename T, int DH>
 int launch_paged(const PagedArgs& a, const Plan& p, long items, hipStream_t st) {
+    constexpr int NW = sizeof(T) == 4 && DH > 64 ? 4 : 8;               // with shared items (plan_of)
     MGX_REQUIRE(items < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
-    // (own rows past 32 make the batch's rows past 32, so shared own items never meet private prefix items)
-    const int rc = p.wide_o   ? launch_items<T, DH, 1, 1>(a, items, st)
-                   : p.wide_p ? launch_items<T, DH, 1, 0>(a, items, st)
-                              : launch_items<T, DH, 0, 0>(a, items, st);
+    const int rc = p.body_o == 2   ? launch_items<T, DH, 2, 2, NW>(a, items, st)
+                   : p.body_p == 2 ? (p.body_o == 1 ? launch_items<T, DH, 2, 1, NW>(a, items, st)
+                                                    : launch_items<T, DH, 2, 0, NW>(a, items, st))
+                   : p.body_p == 1 || p.body_o == 1 ? launch_items<T, DH, 1, 1, 4>(a, items, st)
+                                                    : launch_items<T, DH, 0, 0, 4>(a, items, st);
     if (rc) return rc;
     // (ragged rows in a direct launch: the join kernel clears the rows of no sequence)
     if (a.share || a.So > 1 || a.cu) {
