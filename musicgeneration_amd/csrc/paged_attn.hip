@@ -31,7 +31,7 @@ struct PagedArgs {
     long T, qs;                                   // rows, elements from one row of q to the next
     float scale;
     // plan
-    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, n_items_p;
+    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o;
 };
 
 // sequence, row in it, rows of it, whether row t belongs to one
@@ -646,7 +646,8 @@ __device__ __forceinline__ void put4(T* p, const float* x) {
 }
 
 struct Item {
-    bool prefix, direct;         // prefix: rows of the whole batch; direct: the output itself, nothing to join
+    bool prefix;                 // rows of the whole batch, prefix keys
+    bool direct, fold;           // direct: writes the output itself; fold: takes the prefix's parts in before that
     int b, hk, rt, rts, split;   // row tile and tiles in the grid; split: slot among the parts that are joined
     int k0, k1, n, own;          // key range, rows of the sequence, own keys
     long row0;                   // first row (of q) of the sequence
@@ -668,7 +669,8 @@ __device__ __forceinline__ bool own_item(const PagedArgs& a, int id, Item& it) {
         it.n = (int)(min(max((long)a.cu[it.b + 1], it.row0), a.T) - it.row0);
     }
     it.own = min(max(a.lens[it.b], 0), a.width * a.page);
-    it.direct = !a.share && a.So == 1;
+    it.direct = a.So == 1;
+    it.fold = it.direct && a.share;
     const int base = a.share ? a.P : 0, end = a.P + it.own;
     // ranges of chunk_o keys, the last one open: it takes what a longer sequence than announced has left
     it.k0 = base + it.split * a.chunk_o;
@@ -684,7 +686,7 @@ __device__ __forceinline__ void prefix_item(const PagedArgs& a, int id, Item& it
     // the row tiles of one (head, range) on one XCD (workgroup n runs on XCD n % 8), so that its L2 serves all but the first
     const int pairs = a.Hkv * a.Sp, x = id & 7, rest = id >> 3;
     it.prefix = true;
-    it.direct = false;
+    it.direct = it.fold = false;
     it.rts = a.rt_p;
     it.rt = rest % a.rt_p;
     const int pair = (rest / a.rt_p) * 8 + x;
@@ -715,6 +717,22 @@ __device__ __forceinline__ const T* item_row(const PagedArgs& a, const Item& it,
         limit = max(at, a.P - 1);
     }
     return (const T*)a.q + t * a.qs + (long)h * a.dh;
+}
+
+// parts s0 .. s1-1 of output row `row`, values d0 .. d0+3, onto (maximum, sum, values)
+__device__ __forceinline__ void fold_parts(const PagedArgs& a, long row, int d0, int s0, int s1, float& mm, float& den, float (&x)[4]) {
+    const long step = a.T * a.Hq;
+#pragma unroll 4
+    for (int s = s0; s < s1; ++s) {
+        const long slot = s * step + row;
+        const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
+        const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
+        mm = mn;
+        den = den * f0 + l * f1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
+    }
 }
 
 template <typename T, int DH, int RT, int NW>
@@ -802,6 +820,7 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
                 for (int k = 0; k < 4; ++k) x[k] = fmaf(p[k], f, x[k]);
             }
             const long orow = tt * a.Hq + it.hk * G + rho % G;
+            if (it.fold) fold_parts(a, orow, d0, 0, a.Sp, mm, den, x);
             if (it.direct) {
                 const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
@@ -848,44 +867,74 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
         if (tid < 2) odd_tile[tid] = 0;
         Stage<P_, T, DH, 64, NW> st(lane, w);
         const bool whole = a.dh == DH;
-        unsigned kr = NONE;
         unsigned long long seen = 0, seen_next = 0;
-        // tiles are walked from the last one back (see attn_mfma.hip: with slopes the largest scores come first)
+        // tiles are walked from the last one back (see attn_mfma.hip: with slopes the largest scores come first); at step n
+        // tile n is consumed, n + 1 filed in LDS, n + 2 fetched and the page numbers of n + 3 looked up
         auto tile_of = [&](int n) { return it.k0 + (ntiles - 1 - n) * 64; };
-        auto fetch = [&](int n) {
-            kr = key_row(a, own, it.hk, tile_of(n) + lane, end);
-            st.load(a, kr, whole);
-        };
-        auto file = [&](int n) {
+        auto lookup = [&](int n) { return n < ntiles ? key_row(a, own, it.hk, tile_of(n) + lane, end) : NONE; };
+        auto file = [&](int n, unsigned kr) {
             seen_next = __ballot(kr != NONE);
             if (seen_next != ~0ull || !whole) st.clean(a, kr);
             char* B = smem + (n & 1) * TB;
             if (tile_of(n) + 63 >= sure && st.v_not_finite() && lane == 0) odd_tile[n & 1] = n + 1;
             st.store(B, B + 2 * P_::KB);
         };
+        unsigned kr = lookup(0), kr_next = lookup(1);
         __syncthreads();
         if (ntiles > 0) {
-            fetch(0);
-            file(0);
+            st.load(a, kr, whole);
+            file(0, kr);
             seen = seen_next;
-            if (ntiles > 1) fetch(1);
+            kr = kr_next;
+            kr_next = lookup(2);
+            if (ntiles > 1) st.load(a, kr, whole);
         }
         __syncthreads();
         for (int n = 0; n < ntiles; ++n) {
             const int j0 = tile_of(n);
-            if (n + 1 < ntiles) file(n + 1);
-            if (n + 2 < ntiles) fetch(n + 2);
+            if (n + 1 < ntiles) file(n + 1, kr);
+            if (n + 2 < ntiles) {
+                kr = kr_next;
+                st.load(a, kr, whole);
+                kr_next = lookup(n + 3);
+            }
             const char* B = smem + (n & 1) * TB;
             if (j0 <= rows.last_limit)                                  // uniform in the wave
                 rows.template take<2>(pr, B, B + 2 * P_::KB, j0, seen, odd_tile[n & 1] == n + 1, a.slopes != nullptr, h5);
             seen = seen_next;
             __syncthreads();
         }
-        const float lt = half_swap_sum(rows.l);
+        float den = half_swap_sum(rows.l);
         if (row) {
-            const long orow = t * a.Hq + h;
-            const long slot = (long)it.split * a.T * a.Hq + orow;
-            const float inv = it.direct ? (lt == 0.f ? 0.f : 1.f / lt) : 1.f;
+            const long orow = t * a.Hq + h, step = a.T * a.Hq;
+            float mm = rows.m * rows.c;
+            if (it.fold) {                                              // join the prefix's parts here
+                const float mo = mm;
+                for (int s = 0; s < a.Sp; ++s) mm = fmaxf(mm, a.ml[2 * (s * step + orow)]);
+                const float fo = fast_exp2(mo - mm);
+                den *= fo;
+#pragma unroll
+                for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) rows.o[d][r] *= fo;
+                for (int s = 0; s < a.Sp; ++s) {
+                    const long slot = s * step + orow;
+                    const float f = fast_exp2(a.ml[2 * slot] - mm);
+                    den = fmaf(a.ml[2 * slot + 1], f, den);
+#pragma unroll
+                    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int d0 = 32 * d + 8 * g + 4 * h5;
+                            if (d0 >= a.dh) continue;
+                            const f32x4 x = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) rows.o[d][4 * g + k] = fmaf(x[k], f, rows.o[d][4 * g + k]);
+                        }
+                }
+            }
+            const long slot = (long)it.split * step + orow;
+            const float inv = it.direct ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
@@ -899,8 +948,8 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
                     else put4(a.acc + slot * a.dh + d0, x);
                 }
             if (!it.direct && h5 == 0) {
-                a.ml[2 * slot] = rows.m * rows.c;
-                a.ml[2 * slot + 1] = lt;
+                a.ml[2 * slot] = mm;
+                a.ml[2 * slot + 1] = den;
             }
         }
     }
@@ -913,28 +962,35 @@ constexpr int body_smem() {
     const int tiles = NW * (Prod16<T, DH>::KB + Prod16<T, DH>::VB), rows = BODY == 1 ? 32 : 16, join = NW * rows * (DH + 4 + 2) * 4;
     return tiles > join ? tiles : join;
 }
-template <typename T, int DH, int BODY, int NW>
-__device__ __forceinline__ void body(const PagedArgs& a, const Item& it, char* smem) {
-    if constexpr (BODY == 2) shared_item<T, DH, NW>(a, it, smem);
-    else private_item<T, DH, BODY + 1, NW>(a, it, smem);
+// rows of no sequence (ragged rows before the first or behind the last one): zeros, 64 workgroups
+constexpr int CLEARERS = 64;
+template <typename T>
+__device__ __forceinline__ void clear_rows(const PagedArgs& a, int wg) {
+    const long width = (long)a.Hq * a.dh / 4, first = min(max((long)a.cu[0], 0L), a.T), last = min(max((long)a.cu[a.B], first), a.T);
+    const long n = (first + a.T - last) * width;
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (long e = (long)wg * blockDim.x + threadIdx.x; e < n; e += (long)CLEARERS * blockDim.x)
+        put4((T*)a.out + 4 * (e < first * width ? e : e + (last - first) * width), zero);
 }
 
-template <typename T, int DH, int BODY_P, int BODY_O, int NW>
-__global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a) {
+template <typename T, int DH, int BODY, int NW>
+__global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a, int prefix_pass, int items) {
     extern __shared__ __attribute__((aligned(16))) char paged_smem[];
     Item it;
     const int id = blockIdx.x;
-    if (id < a.n_items_p) {
+    if (id >= items) {
+        clear_rows<T>(a, id - items);
+        return;
+    }
+    if (prefix_pass) {
         prefix_item(a, id, it);
         if (it.hk < 0) return;                                          // (whole workgroups, before any barrier)
-        body<T, DH, BODY_P, NW>(a, it, paged_smem);
-    } else {
-        if (!own_item(a, id - a.n_items_p, it)) return;
-        body<T, DH, BODY_O, NW>(a, it, paged_smem);
-    }
+    } else if (!own_item(a, id, it)) return;
+    if constexpr (BODY == 2) shared_item<T, DH, NW>(a, it, paged_smem);
+    else private_item<T, DH, BODY + 1, NW>(a, it, paged_smem);
 }
 
-// rows of no sequence in a direct launch; every row in a joined one: lanes of 4 values, quads lanes a row
+// the parts of every row joined: 4 values a thread
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
     const int quads = a.dh / 4;
@@ -942,28 +998,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
     if (row >= a.T * a.Hq) return;
     const int d0 = 4 * (int)(e - row * quads);
     int b, r, n;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool real = find_row(a, row / a.Hq, b, r, n);
-    const bool direct = !a.share && a.So == 1;
-    if (direct && real) return;
-    if (real) {
-        const int own = min(max(a.lens[b], 0), a.width * a.page), parts = (a.share ? a.Sp : 0) + own_parts(a, own);
-        const long step = a.T * a.Hq;
-        float mm = NEG, den = 0.f;
-        for (int s = 0; s < parts; ++s) {
-            const long slot = s * step + row;
-            const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
-            const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
-            const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
-            mm = mn;
-            den = den * f0 + l * f1;
+    if (!find_row(a, row / a.Hq, b, r, n)) return;                      // (cleared by the item launch)
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, mm = NEG, den = 0.f;
+    const int own = min(max(a.lens[b], 0), a.width * a.page);
+    fold_parts(a, row, d0, 0, (a.share ? a.Sp : 0) + own_parts(a, own), mm, den, x);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
-        }
-        const float inv = den == 0.f ? 0.f : 1.f / den;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] *= inv;
-    }
+    for (int k = 0; k < 4; ++k) x[k] *= inv;
     put4((T*)a.out + row * a.dh + d0, x);
 }
 
@@ -1040,75 +1081,95 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, 
 // ---- the split: how rows and keys become work items -------------------------------------------------------------------
 struct Plan {
     bool rows_only;                  // the row kernel
-    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, body_p, body_o, nw;
+    int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, body_p, body_o;
 };
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
+// waves of a workgroup: eight (256 rows) for shared items, four where fp32 tiles of dh 128 would pass the LDS
+constexpr int waves_of(int body, int dh, int bytes) { return body == 2 && !(bytes == 4 && dh > 64) ? 8 : 4; }
+
+// Parts of a key range: `base` items of `keys` keys each, of which `slots` workgroups run at once.  A part costs `fix` us of
+// beginning and end and `key` us a key; the parts' sums are written and read again (`row_us` us for all rows of a part),
+// and more than `free` parts need the join launch (4 us).  The cheapest of 1..64.
+inline int parts_of(long base, long keys, long unit, int slots, double fix, double key, double row_us, int free, int& chunk) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64; ++s) {
+        const long c = ceil_div(ceil_div(keys, s), unit) * unit, n = ceil_div(keys, c);
+        if (n != s) continue;
+        const long rounds = ceil_div(base * s, slots);
+        const double cost = rounds * (fix + c * key) + (s > free ? 4.0 : 0.0) + (s > free ? s : 0) * row_us;
+        if (cost < least) least = cost, best = s, chunk = (int)c;
+    }
+    return best;
+}
 
 Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int max_len, int dtype) {
     Plan p = {};
     p.rows_only = dh > 128;                            // a wave's sums, q and staged keys no longer fit its registers
     const long G = Hq / Hkv, rows = (long)max_rows * G;
+    const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : 128;
     auto body_of = [](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : 2; };
-    p.body_o = body_of(rows);
+    auto tile_rows = [&](int body) { return body == 2 ? 32L * waves_of(2, DH, bytes) : 16L * (body + 1); };
     // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
     // sequence whose rows fill a tile by themselves has nothing to gain.
     p.share = P > 0 && B > 1 && T * G < 128L * B;
-    p.body_p = p.share ? body_of(T * G) : p.body_o;
-    if (p.body_p == 1) p.body_o = 1;                   // (one instance fewer: private items of 32 rows take 16, too)
-    if (p.body_o == 2) p.body_p = 2;
-    // shared items: eight waves (256 rows), four where fp32 tiles of dh 128 would pass the LDS
-    p.nw = p.body_p == 2 && !(dtype == MGX_F32 && dh > 64) ? 8 : 4;
-    constexpr long TARGET = 1024;                      // workgroups: two on each of 256 CUs, twice over
-    auto tile_rows = [&](int body) { return body == 2 ? 32L * p.nw : 16L * (body + 1); };
-    auto parts = [&](long base, long keys, int body, int& chunk) {
-        const long unit = body == 2 ? 64 : 32 * p.nw, least = 256;      // fewer keys are all beginning and end
-        long s = ceil_div(TARGET, base);
-        if (s > ceil_div(keys, least)) s = ceil_div(keys, least);
-        if (s < 1) s = 1;
-        chunk = (int)(ceil_div(ceil_div(keys, s), unit) * unit);
-        return (int)ceil_div(keys, chunk);
+    p.body_o = body_of(rows);
+    p.body_p = body_of(T * G);
+    const double row_us = T * Hq * (dh + 2.0) * 8.0 / 5.0e6;              // one part of every row, written and read
+    const long key_bytes = 2L * dh * bytes;
+    auto parts = [&](long base, long keys, int body, int free, int& chunk) {
+        if (body == 2) {                               // compute: about 1.3 us for 64 keys of dh 128 against 256 rows
+            const double key = 0.01 * DH / 128 * (bytes == 4 ? 8 : 1) + 0.01;
+            return parts_of(base, keys, 64, 256, 5.0, key, row_us, free, chunk);
+        }
+        const int slots = 512;                         // two workgroups a CU: 25 bytes/ns each alone, 5 TB/s together
+        const double rate = 5.0e6 / (double)(base < slots ? (base > 200 ? base : 200) : slots);
+        return parts_of(base, keys, 128, slots, 4.0, key_bytes / rate, row_us, free, chunk);
     };
     p.rt_o = (int)ceil_div(rows, tile_rows(p.body_o));
-    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, p.chunk_o);
+    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, 1, p.chunk_o);
     if (p.share) {
         p.rt_p = (int)ceil_div(T * G, tile_rows(p.body_p));
-        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, p.chunk_p);
+        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, 0, p.chunk_p);
     }
     return p;
 }
 
-template <typename T, int DH, int BODY_P, int BODY_O, int NW>
-int launch_items(const PagedArgs& a, long items, hipStream_t st) {
-    constexpr int sp = body_smem<T, DH, BODY_P, NW>(), so = body_smem<T, DH, BODY_O, NW>(), smem = sp > so ? sp : so;
+template <typename T, int DH, int BODY>
+int launch_items(const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
+    constexpr int NW = waves_of(BODY, DH, sizeof(T)), smem = body_smem<T, DH, BODY, NW>();
     static_assert(smem <= 160 * 1024, "LDS of a CU");
+    const long grid = items + (a.cu && !prefix_pass ? CLEARERS : 0);
+    MGX_REQUIRE(grid < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
     if (smem > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY_P, BODY_O, NW>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY, NW>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, smem);
         MGX_REQUIRE(e == hipSuccess, MGX_ELAUNCH, "mgx_paged_attn: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O, NW>), dim3((unsigned)items), dim3(64 * NW), smem, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY, NW>), dim3((unsigned)grid), dim3(64 * NW), smem, st, a, prefix_pass ? 1 : 0,
+                       (int)items);
     MGX_CHECK_LAUNCH("paged_attn");
     return MGX_OK;
 }
+template <typename T, int DH>
+int launch_body(int body, const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
+    return body == 2   ? launch_items<T, DH, 2>(a, prefix_pass, items, st)
+           : body == 1 ? launch_items<T, DH, 1>(a, prefix_pass, items, st)
+                       : launch_items<T, DH, 0>(a, prefix_pass, items, st);
+}
 
 template <typename T, int DH>
-int launch_paged(const PagedArgs& a, const Plan& p, long items, hipStream_t st) {
-    constexpr int NW = sizeof(T) == 4 && DH > 64 ? 4 : 8;               // with shared items (plan_of)
-    MGX_REQUIRE(items < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
-    const int rc = p.body_o == 2   ? launch_items<T, DH, 2, 2, NW>(a, items, st)
-                   : p.body_p == 2 ? (p.body_o == 1 ? launch_items<T, DH, 2, 1, NW>(a, items, st)
-                                                    : launch_items<T, DH, 2, 0, NW>(a, items, st))
-                   : p.body_p == 1 || p.body_o == 1 ? launch_items<T, DH, 1, 1, 4>(a, items, st)
-                                                    : launch_items<T, DH, 0, 0, 4>(a, items, st);
-    if (rc) return rc;
-    // (ragged rows in a direct launch: the join kernel clears the rows of no sequence)
-    if (a.share || a.So > 1 || a.cu) {
-        const long blocks = ceil_div(a.T * a.Hq * (a.dh / 4), 256);
-        MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
-        hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-        MGX_CHECK_LAUNCH("paged_join");
-    }
+int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
+    int rc = MGX_OK;
+    if (p.share) rc = launch_body<T, DH>(p.body_p, a, true, ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p, st);
+    if (!rc) rc = launch_body<T, DH>(p.body_o, a, false, (long)a.B * a.Hkv * p.rt_o * p.So, st);
+    if (rc || p.So == 1) return rc;
+    const long blocks = ceil_div(a.T * a.Hq * (a.dh / 4), 256);
+    MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
+    hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    MGX_CHECK_LAUNCH("paged_join");
     return MGX_OK;
 }
 
@@ -1119,7 +1180,7 @@ extern "C" long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, 
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || dh <= 0 || max_rows <= 0 || max_len <= 0 || prefix_len < 0) return 0;
     const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
     if (p.rows_only || (!p.share && p.So == 1)) return 0;
-    return (p.So + p.Sp) * T * Hq * (dh + 2L);
+    return ((p.So > 1 ? p.So : 0) + p.Sp) * T * Hq * (dh + 2L);
 }
 
 extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const void* vcache, const int* table,
@@ -1164,10 +1225,7 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
         return MGX_OK;
     }
     a.acc = workspace;
-    a.ml = workspace + (p.So + p.Sp) * T * Hq * (long)dh;
-    a.n_items_p = p.share ? (int)(ceil_div((long)Hkv * p.Sp, 8) * 8 * p.rt_p) : 0;
-    MGX_REQUIRE(!p.share || ceil_div((long)Hkv * p.Sp, 8) * 8 * p.rt_p < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
-    const long items = a.n_items_p + (long)B * Hkv * p.rt_o * p.So;
-    if (dtype == MGX_F32) return dh <= 64 ? launch_paged<float, 64>(a, p, items, st) : launch_paged<float, 128>(a, p, items, st);
-    return dh <= 64 ? launch_paged<bf16_t, 64>(a, p, items, st) : launch_paged<bf16_t, 128>(a, p, items, st);
+    a.ml = workspace + ((p.So > 1 ? p.So : 0) + p.Sp) * T * Hq * (long)dh;
+    if (dtype == MGX_F32) return dh <= 64 ? launch_paged<float, 64>(a, p, st) : launch_paged<float, 128>(a, p, st);
+    return dh <= 64 ? launch_paged<bf16_t, 64>(a, p, st) : launch_paged<bf16_t, 128>(a, p, st);
 }
