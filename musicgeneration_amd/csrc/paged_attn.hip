@@ -86,56 +86,59 @@ template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; i
     __device__ static __forceinline__ int koff(int row, int ch) { return Img<DH>::off(row, ch); }
     __device__ static __forceinline__ int voff(int row, int ch) { return Img<DH>::off(row, ch); }
     __device__ static __forceinline__ int qchunk(int ks, int h5) { return 2 * ks + h5; }
-    __device__ __forceinline__ f32x16 scores(const char* K, const QFrag (&q)[NQ], f32x16 s) const {
+    // Fragments are read a group ahead of the products (left alone, the compiler reads one, waits for it and multiplies: an
+    // LDS latency per product), the first V fragments before the softmax.
+    template <int NB>
+    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[NQ], f32x16 (&s)[NB]) const {
+        constexpr int GR = 4, NG = NB * NQ / GR;        // groups of four fragments, one group ahead
+        bf16x8 k[2][GR];
+        auto read = [&](int gr) {
 #pragma unroll
-        for (int ks = 0; ks < NQ; ++ks)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read16(K + la.row_read(0, ks)), q[ks], s, 0, 0, 0);
-        return s;
+            for (int i = 0; i < GR; ++i) k[gr & 1][i] = lds_read16(K + la.row_read((gr * GR + i) / NQ, (gr * GR + i) % NQ));
+        };
+        read(0);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+            if (gr + 1 < NG) read(gr + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < GR; ++i)
+                s[(gr * GR + i) / NQ] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[gr & 1][i], q[(gr * GR + i) % NQ], s[(gr * GR + i) / NQ], 0, 0, 0);
+        }
+    }
+    struct VAhead {
+        bf16x8 f[DH / 32];
+    };
+    __device__ __forceinline__ VAhead vread(const char* V, int tb, int s2) const {
+        VAhead v;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d) v.f[d] = lds_read_tr_pair(V + la.tr_read(tb, s2, 0, d), V + la.tr_read(tb, s2, 1, d));
+        return v;
     }
     // P is rounded to bf16 for the product (2^-8 relative each, signs independent); its sum is taken before that
-    __device__ __forceinline__ void weigh(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
+    template <int NB>
+    __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32]) const {
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            const bf16x8 pf = pack8(p, 8 * s2);
-#pragma unroll
-            for (int d = 0; d < DH / 32; ++d)
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    lds_read_tr_pair(V + la.tr_read(0, s2, 0, d), V + la.tr_read(0, s2, 1, d)), pf, o[d], 0, 0, 0);
-        }
-    }
-    // weigh, where some V value is not finite: such values are left out, and a second product of P with their places (1
-    // there, 0 elsewhere) tells which rows give them weight: those become NaN there, the other rows never meet 0 x inf
-    __device__ __forceinline__ void weigh_odd(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
-#pragma unroll
-        for (int d = 0; d < DH / 32; ++d) {
-            f32x16 z;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = 0.f;
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const bf16x8 pf = pack8(p, 8 * s2);
-                bf16x8 vf = lds_read_tr_pair(V + la.tr_read(0, s2, 0, d), V + la.tr_read(0, s2, 1, d)), at;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const bf16_t x = vf[k];            // (bit_cast of a vector-element lvalue reads element 0)
-                    const bool bad = (__builtin_bit_cast(unsigned short, x) & 0x7F80) == 0x7F80;
-                    at[k] = (bf16_t)(bad ? 1.f : 0.f);
-                    vf[k] = bad ? (bf16_t)0.f : x;
-                }
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[d], 0, 0, 0);
-                z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at, pf, z, 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = z[r] > 0.f ? __builtin_nanf("") : o[d][r];
+        for (int step = 0; step < 2 * NB; ++step) {
+            VAhead next = now;
+            if (step + 1 < 2 * NB) next = vread(V, (step + 1) >> 1, (step + 1) & 1);
+            const bf16x8 pf = pack8(p[step >> 1], 8 * (step & 1));
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.f[d], pf, o[d], 0, 0, 0);
+            now = next;
         }
     }
-    __device__ static __forceinline__ bool not_finite(const f32x4& x) {
+    // values that are not finite become 0; whether there was one
+    __device__ static __forceinline__ bool finite_only(f32x4& x) {
         bool bad = false;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const unsigned w = __float_as_uint(x[k]);
-            bad |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+            unsigned w = __float_as_uint(x[k]);
+            const bool lo = (w & 0x7F80u) == 0x7F80u, hi = (w & 0x7F800000u) == 0x7F800000u;
+            w = (lo ? 0u : w & 0xFFFFu) | (hi ? 0u : w & 0xFFFF0000u);
+            x[k] = __uint_as_float(w);
+            bad |= lo || hi;
         }
         return bad;
     }
@@ -154,45 +157,38 @@ template <int DH> struct Prod<float, DH> {        // v_mfma_f32_32x32x2_f32: the
     __device__ static __forceinline__ int voff(int row, int ch) { return row * VS * 4 + 16 * ch; }
     // the reduced index may be taken in any order: half-wave h5 owns chunk 2 c + h5, four steps of one value each
     __device__ static __forceinline__ int qchunk(int ks, int h) { return 2 * ks + h; }
-    __device__ __forceinline__ f32x16 scores(const char* K, const QFrag (&q)[NQ], f32x16 s) const {
+    template <int NB>
+    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[NQ], f32x16 (&s)[NB]) const {
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-            const f32x4 k = *reinterpret_cast<const f32x4*>(K + koff(l31, 2 * c + h5));
+        for (int c = 0; c < NQ; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[c][e], s, 0, 0, 0);
-        }
-        return s;
+            for (int tb = 0; tb < NB; ++tb) {
+                const f32x4 k = *reinterpret_cast<const f32x4*>(K + tb * KB + koff(l31, 2 * c + h5));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[tb] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[c][e], s[tb], 0, 0, 0);
+            }
     }
-    __device__ __forceinline__ void weigh(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
+    struct VAhead {};
+    __device__ __forceinline__ VAhead vread(const char*, int, int) const { return {}; }
+    template <int NB>
+    __device__ __forceinline__ void weigh(const char* V, VAhead, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32]) const {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float* v = reinterpret_cast<const float*>(V) + (8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31;
-#pragma unroll
-            for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], p[r], o[d], 0, 0, 0);
-        }
-    }
-    __device__ __forceinline__ void weigh_odd(const char* V, const f32x16& p, f32x16 (&o)[DH / 32]) const {
-#pragma unroll
-        for (int d = 0; d < DH / 32; ++d) {
-            f32x16 z;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = 0.f;
+        for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float v = reinterpret_cast<const float*>(V)[(8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31 + 32 * d];
-                const bool bad = (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(bad ? 0.f : v, p[r], o[d], 0, 0, 0);
-                z = __builtin_amdgcn_mfma_f32_32x32x2f32(bad ? 1.f : 0.f, p[r], z, 0, 0, 0);
-            }
+                const float* v = reinterpret_cast<const float*>(V + tb * VB) + (8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = z[r] > 0.f ? __builtin_nanf("") : o[d][r];
-            __builtin_amdgcn_sched_barrier(0);
-        }
+                for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], p[tb][r], o[d], 0, 0, 0);
+            }
     }
-    __device__ static __forceinline__ bool not_finite(const f32x4& x) {
+    __device__ static __forceinline__ bool finite_only(f32x4& x) {
         bool bad = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) bad |= (__float_as_uint(x[k]) & 0x7F800000u) == 0x7F800000u;
+        for (int k = 0; k < 4; ++k) {
+            const bool is = (__float_as_uint(x[k]) & 0x7F800000u) == 0x7F800000u;
+            x[k] = is ? 0.f : x[k];
+            bad |= is;
+        }
         return bad;
     }
 };
@@ -214,24 +210,38 @@ template <int DH> struct Prod16<bf16_t, DH> {     // v_mfma_f32_16x16x32_bf16
     }
     __device__ static __forceinline__ int voff(int row, int ch) { return koff(row, ch); }
     __device__ static __forceinline__ void piece(int lane, int& row, int& ch) { Prod<bf16_t, DH>::piece(lane, row, ch); }
-    __device__ static __forceinline__ bool not_finite(const f32x4& x) { return Prod<bf16_t, DH>::not_finite(x); }
+    __device__ static __forceinline__ bool finite_only(f32x4& x) { return Prod<bf16_t, DH>::finite_only(x); }
     __device__ __forceinline__ Prod16(int lane) {
         const int l15 = lane & 15, g = lane >> 4, q = l15 >> 2, p = l15 & 3;
         k0 = koff(l15, g);
         v0 = koff(4 * g + q, p >> 1) + 8 * (p & 1);
     }
     __device__ static __forceinline__ int qchunk(int ks, int g) { return 4 * ks + g; }
-    // keys 16 kt + .. against the rows of q
+    // keys 16 kt + .. against the rows of q (fragments ahead of the products: see Prod)
     template <int RT>
     __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[RT][NQ], f32x4 (&s)[RT][2]) const {
+        bf16x8 k[NQ][2];
 #pragma unroll
         for (int ks = 0; ks < NQ; ++ks)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const bf16x8 k = lds_read16(K + k0 + 2 * G8 * kt + 512 * ks);
+            for (int kt = 0; kt < 2; ++kt) k[ks][kt] = lds_read16(K + k0 + 2 * G8 * kt + 512 * ks);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[rt][ks], s[rt][kt], 0, 0, 0);
-            }
+        for (int ks = 0; ks < NQ; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[ks][kt], q[rt][ks], s[rt][kt], 0, 0, 0);
+    }
+    static constexpr int AH = 4;                  // V fragments read ahead
+    struct VAhead {
+        bf16x8 f[AH];
+    };
+    __device__ __forceinline__ VAhead vread(const char* V, int d0) const {
+        VAhead v;
+#pragma unroll
+        for (int d = 0; d < AH; ++d) v.f[d] = vfrag(V, d0 + d);
+        return v;
     }
     __device__ static __forceinline__ bf16x8 pack(const f32x4 (&p)[2]) {
         bf16x8 r;
@@ -245,39 +255,21 @@ template <int DH> struct Prod16<bf16_t, DH> {     // v_mfma_f32_16x16x32_bf16
     }
     // P is rounded to bf16 for the product (2^-8 relative each, signs independent); its sum is taken before that
     template <int RT>
-    __device__ __forceinline__ void weigh(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
+    __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
         bf16x8 pf[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) pf[rt] = pack(p[rt]);
 #pragma unroll
-        for (int d = 0; d < DH / 16; ++d) {
-            const bf16x8 v = vfrag(V, d);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[rt], o[rt][d], 0, 0, 0);
-        }
-    }
-    // as Prod::weigh_odd
-    template <int RT>
-    __device__ __forceinline__ void weigh_odd(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
-#pragma unroll
-        for (int d = 0; d < DH / 16; ++d) {
-            bf16x8 v = vfrag(V, d), at;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const bf16_t x = v[k];                 // (bit_cast of a vector-element lvalue reads element 0)
-                const bool bad = (__builtin_bit_cast(unsigned short, x) & 0x7F80) == 0x7F80;
-                at[k] = (bf16_t)(bad ? 1.f : 0.f);
-                v[k] = bad ? (bf16_t)0.f : x;
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const bf16x8 pf = pack(p[rt]);
-                const f32x4 z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at, pf, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf, o[rt][d], 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[rt][d][r] = z[r] > 0.f ? __builtin_nanf("") : o[rt][d][r];
-            }
+        for (int d0 = 0; d0 < DH / 16; d0 += AH) {
+            VAhead next = now;
+            if (d0 + AH < DH / 16) next = vread(V, d0 + AH);
             __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < AH; ++d)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    o[rt][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(now.f[d], pf[rt], o[rt][d0 + d], 0, 0, 0);
+            now = next;
         }
     }
 };
@@ -293,7 +285,7 @@ template <int DH> struct Prod16<float, DH> {      // v_mfma_f32_16x16x4_f32
     __device__ static __forceinline__ int koff(int row, int ch) { return row * DH * 4 + 16 * (ch ^ (row & 15)); }
     __device__ static __forceinline__ int voff(int row, int ch) { return row * VS * 4 + 16 * ch; }
     __device__ static __forceinline__ void piece(int lane, int& row, int& ch) { row = lane >> 3, ch = lane & 7; }
-    __device__ static __forceinline__ bool not_finite(const f32x4& x) { return Prod<float, DH>::not_finite(x); }
+    __device__ static __forceinline__ bool finite_only(f32x4& x) { return Prod<float, DH>::finite_only(x); }
     __device__ static __forceinline__ int qchunk(int ks, int g_) { return 4 * ks + g_; }
     template <int RT>
     __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[RT][NQ], f32x4 (&s)[RT][2]) const {
@@ -312,8 +304,10 @@ template <int DH> struct Prod16<float, DH> {      // v_mfma_f32_16x16x4_f32
     __device__ __forceinline__ float value(const char* V, int kt, int r, int d) const {
         return reinterpret_cast<const float*>(V)[(16 * kt + 4 * g + r) * VS + l15 + 16 * d];
     }
+    struct VAhead {};
+    __device__ __forceinline__ VAhead vread(const char*, int) const { return {}; }
     template <int RT>
-    __device__ __forceinline__ void weigh(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
+    __device__ __forceinline__ void weigh(const char* V, VAhead, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -324,27 +318,6 @@ template <int DH> struct Prod16<float, DH> {      // v_mfma_f32_16x16x4_f32
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[rt][kt][r], o[rt][d], 0, 0, 0);
                 }
-    }
-    template <int RT>
-    __device__ __forceinline__ void weigh_odd(const char* V, const f32x4 (&p)[RT][2], f32x4 (&o)[RT][DH / 16]) const {
-#pragma unroll
-        for (int d = 0; d < DH / 16; ++d)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                f32x4 z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float v = value(V, kt, r, d);
-                        const bool bad = (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 0.f : v, p[rt][kt][r], o[rt][d], 0, 0, 0);
-                        z = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 1.f : 0.f, p[rt][kt][r], z, 0, 0, 0);
-                    }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[rt][d][r] = z[r] > 0.f ? __builtin_nanf("") : o[rt][d][r];
-                __builtin_amdgcn_sched_barrier(0);
-            }
     }
 };
 
@@ -387,10 +360,10 @@ struct Stage {
             v[n] = keep ? v[n] : z;
         }
     }
-    __device__ __forceinline__ bool v_not_finite() const {
+    __device__ __forceinline__ bool v_finite_only() {
         bool bad = false;
 #pragma unroll
-        for (int n = 0; n < N; ++n) bad |= P_::not_finite(v[n]);
+        for (int n = 0; n < N; ++n) bad |= P_::finite_only(v[n]);
         return __any(bad);
     }
     __device__ __forceinline__ void store(char* K, char* V) const {
@@ -448,24 +421,17 @@ struct Rows {
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     }
-    // NB blocks of 32 keys from j0 on; seen: the keys that are somewhere; odd: some V value is not finite
-    template <int NB>
-    __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned long long seen, bool odd,
-                                         bool alibi, int h5) {
+    // NB blocks of 32 keys from j0 on; seen: the keys that are somewhere
+    template <int NB, bool ALIBI>
+    __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned long long seen, int h5) {
         f32x16 s[NB];
+        const float lb = ALIBI ? bias * (float)(j0 + 4 * h5 - at) : 0.f;
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[tb][r] = 0.f;
-        if (alibi) {
-            const float lb = bias * (float)(j0 + 4 * h5 - at);
-#pragma unroll
-            for (int tb = 0; tb < NB; ++tb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[tb][r] = lb + bias * (float)(32 * tb + (r & 3) + 8 * (r >> 2));
-        }
-#pragma unroll
-        for (int tb = 0; tb < NB; ++tb) s[tb] = pr.scores(K + tb * P_::KB, q, s[tb]);
+            for (int r = 0; r < 16; ++r) s[tb][r] = ALIBI ? fmaf(bias, (float)(32 * tb + (r & 3) + 8 * (r >> 2)), lb) : 0.f;
+        pr.template scores<NB>(K, q, s);
+        const typename P_::VAhead va = pr.vread(V, 0, 0);
         const unsigned long long all = NB == 2 ? ~0ull : 0xFFFFFFFFull;
         if (seen != all || j0 + 32 * NB - 1 > first_limit) {          // uniform
             const int dj = limit - j0 - 4 * h5;
@@ -506,17 +472,21 @@ struct Rows {
                 sum += s[tb][r];
             }
         l += sum;
-        if (!odd) {
+        pr.template weigh<NB>(V, va, s, o);
+    }
+    // Keys j0 .. j0+31, whose V values that are not finite were left out: rows that see such a key get NaN there.
+    __device__ __forceinline__ void spoil(const PagedArgs& a, const int* own, int hk, int j0, int end, int h5) {
+        for (int j = j0; j < min(j0 + 32, end); ++j) {
+            const unsigned kr = key_row(a, own, hk, j, end);
+            if (kr == NONE) continue;
+            const T* v = (const T*)a.vc + (size_t)kr * a.dh;
 #pragma unroll
-            for (int tb = 0; tb < NB; ++tb) pr.weigh(V + tb * P_::VB, s[tb], o);
-        } else {
-            int nothing = 0;      // (keeps the compiler from reading the fragments of both branches ahead of them: 64 registers)
-            asm volatile("" : "+s"(nothing));
+            for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
-            for (int tb = 0; tb < NB; ++tb) {
-                pr.weigh_odd(V + tb * P_::VB + nothing, s[tb], o);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const int at_d = 32 * d + 8 * (r >> 2) + 4 * h5 + (r & 3);
+                    if (at_d < a.dh && j <= limit && !(fabsf(to_f32(v[at_d])) < INFINITY)) o[d][r] = __builtin_nanf("");
+                }
         }
     }
 };
@@ -565,21 +535,18 @@ struct Rows16 {
         for (int d = 0; d < DH / 16; ++d) o[rt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     // 32 keys from j0 on (see Rows::take)
-    __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned seen, bool odd, bool alibi,
-                                         int g) {
+    __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned seen, int g) {
         f32x4 s[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (alibi) {
-                    const float lb = bias[rt] * (float)(j0 + 4 * g - at[rt]);
+                const float lb = bias[rt] * (float)(j0 + 4 * g - at[rt]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[rt][kt][r] = lb + bias[rt] * (float)(16 * kt + r);
-                }
+                for (int r = 0; r < 4; ++r) s[rt][kt][r] = fmaf(bias[rt], (float)(16 * kt + r), lb);
             }
         pr.template scores<RT>(K, q, s);
+        const typename P_::VAhead va = pr.vread(V, 0);
         const bool mask = seen != 0xFFFFFFFFu || j0 + 31 > first_limit;          // uniform
         bool grown = false;
         float mx[RT];
@@ -628,8 +595,24 @@ struct Rows16 {
                 }
             l[rt] += sum;
         }
-        if (!odd) pr.template weigh<RT>(V, s, o);
-        else pr.template weigh_odd<RT>(V, s, o);
+        pr.template weigh<RT>(V, va, s, o);
+    }
+    __device__ __forceinline__ void spoil(const PagedArgs& a, const int* own, int hk, int j0, int end, int g) {      // see Rows::spoil
+        for (int j = j0; j < min(j0 + 32, end); ++j) {
+            const unsigned kr = key_row(a, own, hk, j, end);
+            if (kr == NONE) continue;
+            const T* v = (const T*)a.vc + (size_t)kr * a.dh;
+#pragma unroll
+            for (int d = 0; d < DH / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int at_d = 16 * d + 4 * g + r;
+                    const bool bad = at_d < a.dh && !(fabsf(to_f32(v[at_d])) < INFINITY);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        if (bad && j <= limit[rt]) o[rt][d][r] = __builtin_nanf("");
+                }
+        }
     }
 };
 
@@ -758,7 +741,7 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         const int end = min(it.k1, rows.last_limit + 1);
         const bool whole = a.dh == DH;
         Stage<P_, T, DH, 32, 1> st(lane, 0);
-        int j = it.k0 + 32 * w;
+        int j = it.k0 + 32 * w, odd_first = 0x7FFFFFFF, odd_last = -1;
         unsigned kr = key_row(a, own, it.hk, j + l31, end), next = NONE;
         if (j < end) {
             st.load(a, kr, whole);
@@ -767,7 +750,10 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         while (j < end) {
             const unsigned seen = (unsigned)__ballot(kr != NONE);
             if (seen != 0xFFFFFFFFu || !whole) st.clean(a, kr);
-            const bool odd = j + 31 > rows.first_limit && st.v_not_finite();
+            if (j + 31 > rows.first_limit && st.v_finite_only()) {      // (0 x inf must not reach rows that do not see the key)
+                odd_first = min(odd_first, j);
+                odd_last = j;
+            }
             st.store(K, V);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -778,10 +764,11 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
                 st.load(a, kr, whole);
                 next = key_row(a, own, it.hk, j + STEP + l31, end);
             }
-            rows.take(pr, K, V, j0, seen, odd, a.slopes != nullptr, g);
+            rows.take(pr, K, V, j0, seen, g);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
+        for (j = odd_first; j <= odd_last; j += STEP) rows.spoil(a, own, it.hk, j, end, g);
         // join the waves: sums relative to each wave's maximum, through LDS (over the tiles)
         constexpr int LD = DH + 4;
         float* part = reinterpret_cast<float*>(smem);                   // [NW][TR][LD]
@@ -839,7 +826,7 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
     }
 }
 
-template <typename T, int DH, int NW>
+template <typename T, int DH, int NW, bool ALIBI>
 __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod<T, DH> P_;
     constexpr int TB = 2 * (P_::KB + P_::VB);                           // one 64-key buffer: K, then V
@@ -847,7 +834,7 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
     const P_ pr(lane);
-    int* odd_tile = reinterpret_cast<int*>(smem + 2 * TB);              // [2]: 1 + the tile whose V is not finite
+    int* odd = reinterpret_cast<int*>(smem + 2 * TB);                   // first and last key of the tiles with V values left out
     const int* own = a.table + (long)it.b * a.width;
     for (int rt = it.rt; rt * TR < (long)it.n * G; rt += it.rts) {
         long t;
@@ -864,7 +851,7 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             sure = max(p0 + (int)(rt * TR / G), a.P - 1) + 1;
         }
         const int ntiles = end > it.k0 ? (end - it.k0 + 63) / 64 : 0;
-        if (tid < 2) odd_tile[tid] = 0;
+        if (tid == 0) odd[0] = 0x7FFFFFFF, odd[1] = -1;
         Stage<P_, T, DH, 64, NW> st(lane, w);
         const bool whole = a.dh == DH;
         unsigned long long seen = 0, seen_next = 0;
@@ -876,7 +863,10 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             seen_next = __ballot(kr != NONE);
             if (seen_next != ~0ull || !whole) st.clean(a, kr);
             char* B = smem + (n & 1) * TB;
-            if (tile_of(n) + 63 >= sure && st.v_not_finite() && lane == 0) odd_tile[n & 1] = n + 1;
+            if (tile_of(n) + 63 >= sure && st.v_finite_only() && lane == 0) {      // (0 x inf must not reach rows that do not see the key)
+                atomicMin(&odd[0], tile_of(n));
+                atomicMax(&odd[1], tile_of(n) + 63);
+            }
             st.store(B, B + 2 * P_::KB);
         };
         unsigned kr = lookup(0), kr_next = lookup(1);
@@ -900,10 +890,11 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             }
             const char* B = smem + (n & 1) * TB;
             if (j0 <= rows.last_limit)                                  // uniform in the wave
-                rows.template take<2>(pr, B, B + 2 * P_::KB, j0, seen, odd_tile[n & 1] == n + 1, a.slopes != nullptr, h5);
+                rows.template take<2, ALIBI>(pr, B, B + 2 * P_::KB, j0, seen, h5);
             seen = seen_next;
             __syncthreads();
         }
+        for (int j = odd[0]; j <= odd[1]; j += 32) rows.spoil(a, own, it.hk, j, end, h5);
         float den = half_swap_sum(rows.l);
         if (row) {
             const long orow = t * a.Hq + h, step = a.T * a.Hq;
@@ -952,6 +943,7 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
                 a.ml[2 * slot + 1] = den;
             }
         }
+        __syncthreads();                                                // (odd, before the next rows)
     }
 }
 
@@ -973,7 +965,8 @@ __device__ __forceinline__ void clear_rows(const PagedArgs& a, int wg) {
         put4((T*)a.out + 4 * (e < first * width ? e : e + (last - first) * width), zero);
 }
 
-template <typename T, int DH, int BODY, int NW>
+// ALIBI: slopes (shared items; the private ones, which wait for memory, add a slope of 0)
+template <typename T, int DH, int BODY, int NW, bool ALIBI>
 __global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a, int prefix_pass, int items) {
     extern __shared__ __attribute__((aligned(16))) char paged_smem[];
     Item it;
@@ -986,7 +979,7 @@ __global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void page
         prefix_item(a, id, it);
         if (it.hk < 0) return;                                          // (whole workgroups, before any barrier)
     } else if (!own_item(a, id, it)) return;
-    if constexpr (BODY == 2) shared_item<T, DH, NW>(a, it, paged_smem);
+    if constexpr (BODY == 2) shared_item<T, DH, NW, ALIBI>(a, it, paged_smem);
     else private_item<T, DH, BODY + 1, NW>(a, it, paged_smem);
 }
 
@@ -1137,27 +1130,27 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     return p;
 }
 
-template <typename T, int DH, int BODY>
+template <typename T, int DH, int BODY, bool ALIBI>
 int launch_items(const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
     constexpr int NW = waves_of(BODY, DH, sizeof(T)), smem = body_smem<T, DH, BODY, NW>();
     static_assert(smem <= 160 * 1024, "LDS of a CU");
     const long grid = items + (a.cu && !prefix_pass ? CLEARERS : 0);
     MGX_REQUIRE(grid < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
     if (smem > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY, NW>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY, NW, ALIBI>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, smem);
         MGX_REQUIRE(e == hipSuccess, MGX_ELAUNCH, "mgx_paged_attn: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY, NW>), dim3((unsigned)grid), dim3(64 * NW), smem, st, a, prefix_pass ? 1 : 0,
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY, NW, ALIBI>), dim3((unsigned)grid), dim3(64 * NW), smem, st, a, prefix_pass ? 1 : 0,
                        (int)items);
     MGX_CHECK_LAUNCH("paged_attn");
     return MGX_OK;
 }
 template <typename T, int DH>
 int launch_body(int body, const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
-    return body == 2   ? launch_items<T, DH, 2>(a, prefix_pass, items, st)
-           : body == 1 ? launch_items<T, DH, 1>(a, prefix_pass, items, st)
-                       : launch_items<T, DH, 0>(a, prefix_pass, items, st);
+    if (body == 2)
+        return a.slopes ? launch_items<T, DH, 2, true>(a, prefix_pass, items, st) : launch_items<T, DH, 2, false>(a, prefix_pass, items, st);
+    return body == 1 ? launch_items<T, DH, 1, true>(a, prefix_pass, items, st) : launch_items<T, DH, 0, true>(a, prefix_pass, items, st);
 }
 
 template <typename T, int DH>
