@@ -15,7 +15,7 @@
 // operand without leaving the registers (the order of the keys in it is free, V is read in the same one).  Two bodies:
 //   private  <= 16 or 32 rows (16x16 tiles): memory bound.  The waves take alternate 32-key tiles, each through LDS of its
 //            own with the next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
-//   shared   32 rows a wave (32x32 tiles): 64-key tiles in LDS, double buffered, shared by the workgroup.
+//   shared   32 rows a wave (32x32 tiles), 128 in all: 64-key tiles in LDS, double buffered, shared by the four waves.
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
 #include "attn_mfma_common.h"
 
@@ -1079,8 +1079,10 @@ struct Plan {
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// waves of a workgroup: eight (256 rows) for shared items, four where fp32 tiles of dh 128 would pass the LDS
-constexpr int waves_of(int body, int dh, int bytes) { return body == 2 && !(bytes == 4 && dh > 64) ? 8 : 4; }
+// Waves of a workgroup.  Four, two workgroups a CU: against eight (256 rows share a tile, half the reads from L2) prompts of
+// dh 128 take 396 instead of 405 us and those of dh 64 243 instead of 280 - one group's barriers and softmax under the
+// other's products, and a finer end.
+constexpr int NW = 4;
 
 // Parts of a key range: `base` items of `keys` keys each, of which `slots` workgroups run at once.  A part costs `fix` us of
 // beginning and end and `key` us a key; the parts' sums are written and read again (`row_us` us for all rows of a part),
@@ -1104,7 +1106,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     const long G = Hq / Hkv, rows = (long)max_rows * G;
     const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : 128;
     auto body_of = [](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : 2; };
-    auto tile_rows = [&](int body) { return body == 2 ? 32L * waves_of(2, DH, bytes) : 16L * (body + 1); };
+    auto tile_rows = [](int body) { return body == 2 ? 32L * NW : 16L * (body + 1); };
     // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
     // sequence whose rows fill a tile by themselves has nothing to gain.
     p.share = P > 0 && B > 1 && T * G < 128L * B;
@@ -1115,7 +1117,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     auto parts = [&](long base, long keys, int body, int free, int& chunk) {
         if (body == 2) {                               // compute: about 1.3 us for 64 keys of dh 128 against 256 rows
             const double key = 0.01 * DH / 128 * (bytes == 4 ? 8 : 1) + 0.01;
-            return parts_of(base, keys, 64, 256, 5.0, key, row_us, free, chunk);
+            return parts_of(base, keys, 64, 512, 5.0, key, row_us, free, chunk);
         }
         const int slots = 512;                         // two workgroups a CU: 25 bytes/ns each alone, 5 TB/s together
         const double rate = 5.0e6 / (double)(base < slots ? (base > 200 ? base : 200) : slots);
@@ -1132,7 +1134,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
 
 template <typename T, int DH, int BODY, bool ALIBI>
 int launch_items(const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
-    constexpr int NW = waves_of(BODY, DH, sizeof(T)), smem = body_smem<T, DH, BODY, NW>();
+    constexpr int smem = body_smem<T, DH, BODY, NW>();
     static_assert(smem <= 160 * 1024, "LDS of a CU");
     const long grid = items + (a.cu && !prefix_pass ? CLEARERS : 0);
     MGX_REQUIRE(grid < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
