@@ -57,14 +57,19 @@ __device__ __forceinline__ bool find_row(const PagedArgs& a, long t, int& b, int
 constexpr unsigned NONE = 0xFFFFFFFFu;
 constexpr float NEG = -1.0e30f;       // a running maximum before any key: finite, so differences stay numbers
 
-// Where numbered key j of sequence table `own` lies, in rows of the pool; NONE: nowhere (hidden, or not before `end`).
-__device__ __forceinline__ unsigned key_row(const PagedArgs& a, const int* own, int hk, int j, int end) {
-    if (j >= end) return NONE;
+// Where numbered key j lies, in rows of the pool, in two steps, so that the page number is loaded a tile before it is
+// needed (a wait for it where it is loaded would wait for the tile's keys, too): the page's number - of key end - 1 behind
+// the end, so that nothing is masked; end > 0 -, and the row, NONE where the key is hidden or not before `end`.
+__device__ __forceinline__ unsigned page_of(const PagedArgs& a, const int* own, int j, int end) {
+    j = min(j, end - 1);
     const bool pre = j < a.P;
     const int jj = pre ? j : j - a.P;
-    const int p = a.shift >= 0 ? jj >> a.shift : jj / a.page;
-    const unsigned pg = (unsigned)(pre ? a.prefix[p] : own[p]);
-    return pg < (unsigned)a.n_pages ? (pg * a.Hkv + hk) * a.page + (jj - p * a.page) : NONE;
+    return (unsigned)(pre ? a.prefix : own)[a.shift >= 0 ? jj >> a.shift : jj / a.page];
+}
+__device__ __forceinline__ unsigned slot_of(const PagedArgs& a, int hk, unsigned pg, int j, int end) {
+    const int jj = j < a.P ? j : j - a.P;
+    const int in_page = a.shift >= 0 ? jj & (a.page - 1) : jj % a.page;
+    return j < end && pg < (unsigned)a.n_pages ? (pg * a.Hkv + hk) * a.page + in_page : NONE;
 }
 
 // ---- LDS images and matrix products per storage type ------------------------------------------------------------------
@@ -115,14 +120,18 @@ template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; i
         for (int d = 0; d < DH / 32; ++d) v.f[d] = lds_read_tr_pair(V + la.tr_read(tb, s2, 0, d), V + la.tr_read(tb, s2, 1, d));
         return v;
     }
-    // P is rounded to bf16 for the product (2^-8 relative each, signs independent); its sum is taken before that
+    // P is rounded to bf16 for the product (2^-8 relative each, signs independent) and so for the sum, so that the weights
+    // add up to one; two values an instruction
     template <int NB>
-    __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32]) const {
+    __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32], float& l) const {
+        const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
 #pragma unroll
         for (int step = 0; step < 2 * NB; ++step) {
             VAhead next = now;
             if (step + 1 < 2 * NB) next = vread(V, (step + 1) >> 1, (step + 1) & 1);
             const bf16x8 pf = pack8(p[step >> 1], 8 * (step & 1));
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pf[k], pf[k + 1]}, one, l, false);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.f[d], pf, o[d], 0, 0, 0);
@@ -171,11 +180,12 @@ template <int DH> struct Prod<float, DH> {        // v_mfma_f32_32x32x2_f32: the
     struct VAhead {};
     __device__ __forceinline__ VAhead vread(const char*, int, int) const { return {}; }
     template <int NB>
-    __device__ __forceinline__ void weigh(const char* V, VAhead, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32]) const {
+    __device__ __forceinline__ void weigh(const char* V, VAhead, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32], float& l) const {
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
+                l += p[tb][r];
                 const float* v = reinterpret_cast<const float*>(V + tb * VB) + (8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31;
 #pragma unroll
                 for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], p[tb][r], o[d], 0, 0, 0);
@@ -339,7 +349,7 @@ struct Stage {
     // (N is a multiple of W or the other way round, so a wave's requests are a rectangle)
     __device__ __forceinline__ int row(int n) const { return r0 + 8 * (n / W); }
     __device__ __forceinline__ int chunk(int n) const { return c0 + 8 * (n % W); }
-    // at: lane r's key_row of the tile's key r.  Rows that are nowhere read row 0 and are zeroed, so no load is masked.
+    // at: lane r's slot_of the tile's key r.  Rows that are nowhere read row 0 and are zeroed, so no load is masked.
     __device__ __forceinline__ void load(const PagedArgs& a, unsigned at, bool whole) {
         const unsigned bytes = a.dh * (unsigned)sizeof(T);
         const unsigned safe = at == NONE ? 0u : at;
@@ -463,21 +473,16 @@ struct Rows {
                 for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
         }
         const float mc = m * c;
-        float sum = 0.f;
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[tb][r] = fast_exp2(fmaf(s[tb][r], c, -mc));
-                sum += s[tb][r];
-            }
-        l += sum;
-        pr.template weigh<NB>(V, va, s, o);
+            for (int r = 0; r < 16; ++r) s[tb][r] = fast_exp2(fmaf(s[tb][r], c, -mc));
+        pr.template weigh<NB>(V, va, s, o, l);
     }
     // Keys j0 .. j0+31, whose V values that are not finite were left out: rows that see such a key get NaN there.
     __device__ __forceinline__ void spoil(const PagedArgs& a, const int* own, int hk, int j0, int end, int h5) {
         for (int j = j0; j < min(j0 + 32, end); ++j) {
-            const unsigned kr = key_row(a, own, hk, j, end);
+            const unsigned kr = slot_of(a, hk, page_of(a, own, j, end), j, end);
             if (kr == NONE) continue;
             const T* v = (const T*)a.vc + (size_t)kr * a.dh;
 #pragma unroll
@@ -599,7 +604,7 @@ struct Rows16 {
     }
     __device__ __forceinline__ void spoil(const PagedArgs& a, const int* own, int hk, int j0, int end, int g) {      // see Rows::spoil
         for (int j = j0; j < min(j0 + 32, end); ++j) {
-            const unsigned kr = key_row(a, own, hk, j, end);
+            const unsigned kr = slot_of(a, hk, page_of(a, own, j, end), j, end);
             if (kr == NONE) continue;
             const T* v = (const T*)a.vc + (size_t)kr * a.dh;
 #pragma unroll
@@ -742,10 +747,11 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         const bool whole = a.dh == DH;
         Stage<P_, T, DH, 32, 1> st(lane, 0);
         int j = it.k0 + 32 * w, odd_first = 0x7FFFFFFF, odd_last = -1;
-        unsigned kr = key_row(a, own, it.hk, j + l31, end), next = NONE;
+        unsigned kr = NONE, page = 0;
         if (j < end) {
+            kr = slot_of(a, it.hk, page_of(a, own, j + l31, end), j + l31, end);
+            page = page_of(a, own, j + STEP + l31, end);
             st.load(a, kr, whole);
-            next = key_row(a, own, it.hk, j + STEP + l31, end);
         }
         while (j < end) {
             const unsigned seen = (unsigned)__ballot(kr != NONE);
@@ -759,10 +765,10 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
             __builtin_amdgcn_wave_barrier();
             const int j0 = j;
             j += STEP;
-            kr = next;
             if (j < end) {
+                kr = slot_of(a, it.hk, page, j + l31, end);
+                page = page_of(a, own, j + STEP + l31, end);
                 st.load(a, kr, whole);
-                next = key_row(a, own, it.hk, j + STEP + l31, end);
             }
             rows.take(pr, K, V, j0, seen, g);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -858,7 +864,8 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
         // tiles are walked from the last one back (see attn_mfma.hip: with slopes the largest scores come first); at step n
         // tile n is consumed, n + 1 filed in LDS, n + 2 fetched and the page numbers of n + 3 looked up
         auto tile_of = [&](int n) { return it.k0 + (ntiles - 1 - n) * 64; };
-        auto lookup = [&](int n) { return n < ntiles ? key_row(a, own, it.hk, tile_of(n) + lane, end) : NONE; };
+        auto lookup = [&](int n) { return page_of(a, own, max(tile_of(n), it.k0) + lane, end); };
+        auto slot = [&](int n, unsigned page) { return slot_of(a, it.hk, page, tile_of(n) + lane, end); };
         auto file = [&](int n, unsigned kr) {
             seen_next = __ballot(kr != NONE);
             if (seen_next != ~0ull || !whole) st.clean(a, kr);
@@ -869,24 +876,28 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             }
             st.store(B, B + 2 * P_::KB);
         };
-        unsigned kr = lookup(0), kr_next = lookup(1);
+        unsigned kr = NONE, page = 0;
         __syncthreads();
         if (ntiles > 0) {
+            kr = slot(0, lookup(0));
             st.load(a, kr, whole);
+            page = lookup(1);
             file(0, kr);
             seen = seen_next;
-            kr = kr_next;
-            kr_next = lookup(2);
-            if (ntiles > 1) st.load(a, kr, whole);
+            if (ntiles > 1) {
+                kr = slot(1, page);
+                page = lookup(2);
+                st.load(a, kr, whole);
+            }
         }
         __syncthreads();
         for (int n = 0; n < ntiles; ++n) {
             const int j0 = tile_of(n);
             if (n + 1 < ntiles) file(n + 1, kr);
             if (n + 2 < ntiles) {
-                kr = kr_next;
+                kr = slot(n + 2, page);
+                page = lookup(n + 3);
                 st.load(a, kr, whole);
-                kr_next = lookup(n + 3);
             }
             const char* B = smem + (n & 1) * TB;
             if (j0 <= rows.last_limit)                                  // uniform in the wave
