@@ -54,6 +54,10 @@ __device__ __forceinline__ bool find_row(const PagedArgs& a, long t, int& b, int
     return r >= 0 && r < n;
 }
 
+// Waves of a workgroup.  Four, two workgroups a CU: against eight (256 rows share a tile, half the reads from L2) prompts of
+// dh 128 take 396 instead of 405 us and those of dh 64 243 instead of 280 - one group's barriers and softmax under the
+// other's products, and a finer end.
+constexpr int NW = 4;
 constexpr unsigned NONE = 0xFFFFFFFFu;
 constexpr float NEG = -1.0e30f;       // a running maximum before any key: finite, so differences stay numbers
 
@@ -634,8 +638,7 @@ __device__ __forceinline__ void put4(T* p, const float* x) {
 }
 
 struct Item {
-    bool prefix;                 // rows of the whole batch, prefix keys
-    bool direct, fold;           // direct: writes the output itself; fold: takes the prefix's parts in before that
+    bool prefix, direct;         // prefix: rows of the whole batch, prefix keys; direct: the output itself, nothing to join
     int b, hk, rt, rts, split;   // row tile and tiles in the grid; split: slot among the parts that are joined
     int k0, k1, n, own;          // key range, rows of the sequence, own keys
     long row0;                   // first row (of q) of the sequence
@@ -657,8 +660,7 @@ __device__ __forceinline__ bool own_item(const PagedArgs& a, int id, Item& it) {
         it.n = (int)(min(max((long)a.cu[it.b + 1], it.row0), a.T) - it.row0);
     }
     it.own = min(max(a.lens[it.b], 0), a.width * a.page);
-    it.direct = a.So == 1;
-    it.fold = it.direct && a.share;
+    it.direct = !a.share && a.So == 1;
     const int base = a.share ? a.P : 0, end = a.P + it.own;
     // ranges of chunk_o keys, the last one open: it takes what a longer sequence than announced has left
     it.k0 = base + it.split * a.chunk_o;
@@ -674,7 +676,7 @@ __device__ __forceinline__ void prefix_item(const PagedArgs& a, int id, Item& it
     // the row tiles of one (head, range) on one XCD (workgroup n runs on XCD n % 8), so that its L2 serves all but the first
     const int pairs = a.Hkv * a.Sp, x = id & 7, rest = id >> 3;
     it.prefix = true;
-    it.direct = it.fold = false;
+    it.direct = false;
     it.rts = a.rt_p;
     it.rt = rest % a.rt_p;
     const int pair = (rest / a.rt_p) * 8 + x;
@@ -707,23 +709,7 @@ __device__ __forceinline__ const T* item_row(const PagedArgs& a, const Item& it,
     return (const T*)a.q + t * a.qs + (long)h * a.dh;
 }
 
-// parts s0 .. s1-1 of output row `row`, values d0 .. d0+3, onto (maximum, sum, values)
-__device__ __forceinline__ void fold_parts(const PagedArgs& a, long row, int d0, int s0, int s1, float& mm, float& den, float (&x)[4]) {
-    const long step = a.T * a.Hq;
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-        const long slot = s * step + row;
-        const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
-        const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
-        mm = mn;
-        den = den * f0 + l * f1;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
-    }
-}
-
-template <typename T, int DH, int RT, int NW>
+template <typename T, int DH, int RT>
 __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod16<T, DH> P_;
     constexpr int TR = 16 * RT, STEP = 32 * NW;
@@ -813,7 +799,6 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
                 for (int k = 0; k < 4; ++k) x[k] = fmaf(p[k], f, x[k]);
             }
             const long orow = tt * a.Hq + it.hk * G + rho % G;
-            if (it.fold) fold_parts(a, orow, d0, 0, a.Sp, mm, den, x);
             if (it.direct) {
                 const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
@@ -832,7 +817,7 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
     }
 }
 
-template <typename T, int DH, int NW, bool ALIBI>
+template <typename T, int DH, bool ALIBI>
 __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod<T, DH> P_;
     constexpr int TB = 2 * (P_::KB + P_::VB);                           // one 64-key buffer: K, then V
@@ -906,36 +891,10 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             __syncthreads();
         }
         for (int j = odd[0]; j <= odd[1]; j += 32) rows.spoil(a, own, it.hk, j, end, h5);
-        float den = half_swap_sum(rows.l);
+        const float den = half_swap_sum(rows.l);
         if (row) {
-            const long orow = t * a.Hq + h, step = a.T * a.Hq;
-            float mm = rows.m * rows.c;
-            if (it.fold) {                                              // join the prefix's parts here
-                const float mo = mm;
-                for (int s = 0; s < a.Sp; ++s) mm = fmaxf(mm, a.ml[2 * (s * step + orow)]);
-                const float fo = fast_exp2(mo - mm);
-                den *= fo;
-#pragma unroll
-                for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) rows.o[d][r] *= fo;
-                for (int s = 0; s < a.Sp; ++s) {
-                    const long slot = s * step + orow;
-                    const float f = fast_exp2(a.ml[2 * slot] - mm);
-                    den = fmaf(a.ml[2 * slot + 1], f, den);
-#pragma unroll
-                    for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const int d0 = 32 * d + 8 * g + 4 * h5;
-                            if (d0 >= a.dh) continue;
-                            const f32x4 x = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) rows.o[d][4 * g + k] = fmaf(x[k], f, rows.o[d][4 * g + k]);
-                        }
-                }
-            }
-            const long slot = (long)it.split * step + orow;
+            const long orow = t * a.Hq + h;
+            const long slot = (long)it.split * a.T * a.Hq + orow;
             const float inv = it.direct ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d)
@@ -950,7 +909,7 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
                     else put4(a.acc + slot * a.dh + d0, x);
                 }
             if (!it.direct && h5 == 0) {
-                a.ml[2 * slot] = mm;
+                a.ml[2 * slot] = rows.m * rows.c;
                 a.ml[2 * slot + 1] = den;
             }
         }
@@ -959,7 +918,7 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
 }
 
 // BODY: 0 / 1 private with 16 / 32 rows, 2 shared
-template <typename T, int DH, int BODY, int NW>
+template <typename T, int DH, int BODY>
 constexpr int body_smem() {
     if (BODY == 2) return 4 * (Prod<T, DH>::KB + Prod<T, DH>::VB) + 16;
     const int tiles = NW * (Prod16<T, DH>::KB + Prod16<T, DH>::VB), rows = BODY == 1 ? 32 : 16, join = NW * rows * (DH + 4 + 2) * 4;
@@ -977,8 +936,15 @@ __device__ __forceinline__ void clear_rows(const PagedArgs& a, int wg) {
 }
 
 // ALIBI: slopes (shared items; the private ones, which wait for memory, add a slope of 0)
-template <typename T, int DH, int BODY, int NW, bool ALIBI>
-__global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a, int prefix_pass, int items) {
+template <typename T, int DH, int BODY, bool ALIBI>
+__device__ __forceinline__ void run_item(const PagedArgs& a, const Item& it, char* smem) {
+    if constexpr (BODY == 2) shared_item<T, DH, ALIBI>(a, it, smem);
+    else private_item<T, DH, BODY + 1>(a, it, smem);
+}
+// Prefix items first, then own items, in one launch: the former are bound by arithmetic, the latter by memory, and a CU holds
+// one of each.
+template <typename T, int DH, int BODY_P, int BODY_O, bool ALIBI>
+__global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a, int items_p, int items) {
     extern __shared__ __attribute__((aligned(16))) char paged_smem[];
     Item it;
     const int id = blockIdx.x;
@@ -986,12 +952,14 @@ __global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void page
         clear_rows<T>(a, id - items);
         return;
     }
-    if (prefix_pass) {
+    if (id < items_p) {
         prefix_item(a, id, it);
         if (it.hk < 0) return;                                          // (whole workgroups, before any barrier)
-    } else if (!own_item(a, id, it)) return;
-    if constexpr (BODY == 2) shared_item<T, DH, NW, ALIBI>(a, it, paged_smem);
-    else private_item<T, DH, BODY + 1, NW>(a, it, paged_smem);
+        run_item<T, DH, BODY_P, ALIBI>(a, it, paged_smem);
+    } else {
+        if (!own_item(a, id - items_p, it)) return;
+        run_item<T, DH, BODY_O, ALIBI>(a, it, paged_smem);
+    }
 }
 
 // the parts of every row joined: 4 values a thread
@@ -1004,8 +972,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
     int b, r, n;
     if (!find_row(a, row / a.Hq, b, r, n)) return;                      // (cleared by the item launch)
     float x[4] = {0.f, 0.f, 0.f, 0.f}, mm = NEG, den = 0.f;
-    const int own = min(max(a.lens[b], 0), a.width * a.page);
-    fold_parts(a, row, d0, 0, (a.share ? a.Sp : 0) + own_parts(a, own), mm, den, x);
+    const int own = min(max(a.lens[b], 0), a.width * a.page), parts = (a.share ? a.Sp : 0) + own_parts(a, own);
+    const long step = a.T * a.Hq;
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        const long slot = s * step + row;
+        const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
+        const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
+        const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
+        mm = mn;
+        den = den * f0 + l * f1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
+    }
     const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] *= inv;
@@ -1090,22 +1069,17 @@ struct Plan {
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// Waves of a workgroup.  Four, two workgroups a CU: against eight (256 rows share a tile, half the reads from L2) prompts of
-// dh 128 take 396 instead of 405 us and those of dh 64 243 instead of 280 - one group's barriers and softmax under the
-// other's products, and a finer end.
-constexpr int NW = 4;
-
 // Parts of a key range: `base` items of `keys` keys each, of which `slots` workgroups run at once.  A part costs `fix` us of
-// beginning and end and `key` us a key; the parts' sums are written and read again (`row_us` us for all rows of a part),
-// and more than `free` parts need the join launch (4 us).  The cheapest of 1..64.
-inline int parts_of(long base, long keys, long unit, int slots, double fix, double key, double row_us, int free, int& chunk) {
+// beginning and end and `key` us a key; the parts' sums are written and read again (`row_us` us for all rows of a part);
+// `join`: one part alone would need neither that nor the join launch (4 us).  The cheapest of 1..64.
+inline int parts_of(long base, long keys, long unit, int slots, double fix, double key, double row_us, bool join, int& chunk) {
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 64; ++s) {
         const long c = ceil_div(ceil_div(keys, s), unit) * unit, n = ceil_div(keys, c);
         if (n != s) continue;
         const long rounds = ceil_div(base * s, slots);
-        const double cost = rounds * (fix + c * key) + (s > free ? 4.0 : 0.0) + (s > free ? s : 0) * row_us;
+        const double cost = rounds * (fix + c * key) + (s > 1 && join ? 4.0 : 0.0) + (s > 1 || !join ? s : 0) * row_us;
         if (cost < least) least = cost, best = s, chunk = (int)c;
     }
     return best;
@@ -1122,56 +1096,59 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     // sequence whose rows fill a tile by themselves has nothing to gain.
     p.share = P > 0 && B > 1 && T * G < 128L * B;
     p.body_o = body_of(rows);
-    p.body_p = body_of(T * G);
+    p.body_p = p.share ? body_of(T * G) : p.body_o;
+    if (p.body_p == 1 || (p.body_o > p.body_p)) p.body_o = p.body_p;     // (instances: private items of 32 rows take 16, too)
     const double row_us = T * Hq * (dh + 2.0) * 8.0 / 5.0e6;              // one part of every row, written and read
     const long key_bytes = 2L * dh * bytes;
-    auto parts = [&](long base, long keys, int body, int free, int& chunk) {
+    auto parts = [&](long base, long keys, int body, bool join, int& chunk) {
         if (body == 2) {                               // compute: about 1.3 us for 64 keys of dh 128 against 256 rows
             const double key = 0.01 * DH / 128 * (bytes == 4 ? 8 : 1) + 0.01;
-            return parts_of(base, keys, 64, 512, 5.0, key, row_us, free, chunk);
+            return parts_of(base, keys, 64, 512, 5.0, key, row_us, join, chunk);
         }
         const int slots = 512;                         // two workgroups a CU: 25 bytes/ns each alone, 5 TB/s together
         const double rate = 5.0e6 / (double)(base < slots ? (base > 200 ? base : 200) : slots);
-        return parts_of(base, keys, 128, slots, 4.0, key_bytes / rate, row_us, free, chunk);
+        return parts_of(base, keys, 128, slots, 4.0, key_bytes / rate, row_us, join, chunk);
     };
     p.rt_o = (int)ceil_div(rows, tile_rows(p.body_o));
-    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, 1, p.chunk_o);
+    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, !p.share, p.chunk_o);
     if (p.share) {
         p.rt_p = (int)ceil_div(T * G, tile_rows(p.body_p));
-        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, 0, p.chunk_p);
+        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, false, p.chunk_p);
     }
     return p;
 }
 
-template <typename T, int DH, int BODY, bool ALIBI>
-int launch_items(const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
-    constexpr int smem = body_smem<T, DH, BODY, NW>();
+template <typename T, int DH, int BODY_P, int BODY_O, bool ALIBI>
+int launch_items(const PagedArgs& a, long items_p, long items_o, hipStream_t st) {
+    constexpr int sp = body_smem<T, DH, BODY_P>(), so = body_smem<T, DH, BODY_O>(), smem = sp > so ? sp : so;
     static_assert(smem <= 160 * 1024, "LDS of a CU");
-    const long grid = items + (a.cu && !prefix_pass ? CLEARERS : 0);
+    const long items = items_p + items_o, grid = items + (a.cu ? CLEARERS : 0);
     MGX_REQUIRE(grid < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
     if (smem > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY, NW, ALIBI>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY_P, BODY_O, ALIBI>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, smem);
         MGX_REQUIRE(e == hipSuccess, MGX_ELAUNCH, "mgx_paged_attn: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY, NW, ALIBI>), dim3((unsigned)grid), dim3(64 * NW), smem, st, a, prefix_pass ? 1 : 0,
-                       (int)items);
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O, ALIBI>), dim3((unsigned)grid), dim3(64 * NW), smem, st, a,
+                       (int)items_p, (int)items);
     MGX_CHECK_LAUNCH("paged_attn");
     return MGX_OK;
-}
-template <typename T, int DH>
-int launch_body(int body, const PagedArgs& a, bool prefix_pass, long items, hipStream_t st) {
-    if (body == 2)
-        return a.slopes ? launch_items<T, DH, 2, true>(a, prefix_pass, items, st) : launch_items<T, DH, 2, false>(a, prefix_pass, items, st);
-    return body == 1 ? launch_items<T, DH, 1, true>(a, prefix_pass, items, st) : launch_items<T, DH, 0, true>(a, prefix_pass, items, st);
 }
 
 template <typename T, int DH>
 int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
-    int rc = MGX_OK;
-    if (p.share) rc = launch_body<T, DH>(p.body_p, a, true, ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p, st);
-    if (!rc) rc = launch_body<T, DH>(p.body_o, a, false, (long)a.B * a.Hkv * p.rt_o * p.So, st);
-    if (rc || p.So == 1) return rc;
+    const long ip = p.share ? ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p : 0, io = (long)a.B * a.Hkv * p.rt_o * p.So;
+    int rc;
+    if (p.body_p < 2) rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
+    else if (a.slopes)
+        rc = p.body_o == 2   ? launch_items<T, DH, 2, 2, true>(a, ip, io, st)
+             : p.body_o == 1 ? launch_items<T, DH, 2, 1, true>(a, ip, io, st)
+                             : launch_items<T, DH, 2, 0, true>(a, ip, io, st);
+    else
+        rc = p.body_o == 2   ? launch_items<T, DH, 2, 2, false>(a, ip, io, st)
+             : p.body_o == 1 ? launch_items<T, DH, 2, 1, false>(a, ip, io, st)
+                             : launch_items<T, DH, 2, 0, false>(a, ip, io, st);
+    if (rc || (!p.share && p.So == 1)) return rc;
     const long blocks = ceil_div(a.T * a.Hq * (a.dh / 4), 256);
     MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
     hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
@@ -1186,7 +1163,7 @@ extern "C" long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, 
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || dh <= 0 || max_rows <= 0 || max_len <= 0 || prefix_len < 0) return 0;
     const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
     if (p.rows_only || (!p.share && p.So == 1)) return 0;
-    return ((p.So > 1 ? p.So : 0) + p.Sp) * T * Hq * (dh + 2L);
+    return (p.So + p.Sp) * T * Hq * (dh + 2L);
 }
 
 extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const void* vcache, const int* table,
@@ -1231,7 +1208,7 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
         return MGX_OK;
     }
     a.acc = workspace;
-    a.ml = workspace + ((p.So > 1 ? p.So : 0) + p.Sp) * T * Hq * (long)dh;
+    a.ml = workspace + (p.So + p.Sp) * T * Hq * (long)dh;
     if (dtype == MGX_F32) return dh <= 64 ? launch_paged<float, 64>(a, p, st) : launch_paged<float, 128>(a, p, st);
     return dh <= 64 ? launch_paged<bf16_t, 64>(a, p, st) : launch_paged<bf16_t, 128>(a, p, st);
 }
