@@ -97,9 +97,9 @@ template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; i
     __device__ static __forceinline__ int qchunk(int ks, int h5) { return 2 * ks + h5; }
     // Fragments are read a group ahead of the products (left alone, the compiler reads one, waits for it and multiplies: an
     // LDS latency per product), the first V fragments before the softmax.
-    template <int NB>
-    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[NQ], f32x16 (&s)[NB]) const {
-        constexpr int GR = 4, NG = NB * NQ / GR;        // groups of four fragments, one group ahead
+    template <int NB, int RW>
+    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[RW][NQ], f32x16 (&s)[RW][NB]) const {
+        constexpr int GR = 4 / RW, NG = NB * NQ / GR;   // groups of fragments for four or eight products, one group ahead
         bf16x8 k[2][GR];
         auto read = [&](int gr) {
 #pragma unroll
@@ -111,8 +111,11 @@ template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; i
             if (gr + 1 < NG) read(gr + 1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < GR; ++i)
-                s[(gr * GR + i) / NQ] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[gr & 1][i], q[(gr * GR + i) % NQ], s[(gr * GR + i) / NQ], 0, 0, 0);
+            for (int i = 0; i < GR; ++i) {
+                const int tb = (gr * GR + i) / NQ, ks = (gr * GR + i) % NQ;
+#pragma unroll
+                for (int w = 0; w < RW; ++w) s[w][tb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[gr & 1][i], q[w][ks], s[w][tb], 0, 0, 0);
+            }
         }
     }
     struct VAhead {
@@ -126,19 +129,26 @@ template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; i
     }
     // P is rounded to bf16 for the product (2^-8 relative each, signs independent) and so for the sum, so that the weights
     // add up to one; two values an instruction
-    template <int NB>
-    __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32], float& l) const {
+    template <int NB, int RW>
+    __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x16 (&p)[RW][NB], f32x16 (&o)[RW][DH / 32],
+                                          float (&l)[RW]) const {
         const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
 #pragma unroll
         for (int step = 0; step < 2 * NB; ++step) {
             VAhead next = now;
             if (step + 1 < 2 * NB) next = vread(V, (step + 1) >> 1, (step + 1) & 1);
-            const bf16x8 pf = pack8(p[step >> 1], 8 * (step & 1));
+            bf16x8 pf[RW];
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pf[k], pf[k + 1]}, one, l, false);
+            for (int w = 0; w < RW; ++w) {
+                pf[w] = pack8(p[w][step >> 1], 8 * (step & 1));
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) l[w] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pf[w][k], pf[w][k + 1]}, one, l[w], false);
+            }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.f[d], pf, o[d], 0, 0, 0);
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int w = 0; w < RW; ++w) o[w][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.f[d], pf[w], o[w][d], 0, 0, 0);
             now = next;
         }
     }
@@ -170,29 +180,34 @@ template <int DH> struct Prod<float, DH> {        // v_mfma_f32_32x32x2_f32: the
     __device__ static __forceinline__ int voff(int row, int ch) { return row * VS * 4 + 16 * ch; }
     // the reduced index may be taken in any order: half-wave h5 owns chunk 2 c + h5, four steps of one value each
     __device__ static __forceinline__ int qchunk(int ks, int h) { return 2 * ks + h; }
-    template <int NB>
-    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[NQ], f32x16 (&s)[NB]) const {
+    template <int NB, int RW>
+    __device__ __forceinline__ void scores(const char* K, const QFrag (&q)[RW][NQ], f32x16 (&s)[RW][NB]) const {
 #pragma unroll
         for (int c = 0; c < NQ; ++c)
 #pragma unroll
             for (int tb = 0; tb < NB; ++tb) {
                 const f32x4 k = *reinterpret_cast<const f32x4*>(K + tb * KB + koff(l31, 2 * c + h5));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[tb] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[c][e], s[tb], 0, 0, 0);
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int w = 0; w < RW; ++w) s[w][tb] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[w][c][e], s[w][tb], 0, 0, 0);
             }
     }
     struct VAhead {};
     __device__ __forceinline__ VAhead vread(const char*, int, int) const { return {}; }
-    template <int NB>
-    __device__ __forceinline__ void weigh(const char* V, VAhead, const f32x16 (&p)[NB], f32x16 (&o)[DH / 32], float& l) const {
+    template <int NB, int RW>
+    __device__ __forceinline__ void weigh(const char* V, VAhead, const f32x16 (&p)[RW][NB], f32x16 (&o)[RW][DH / 32], float (&l)[RW]) const {
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                l += p[tb][r];
                 const float* v = reinterpret_cast<const float*>(V + tb * VB) + (8 * (r >> 2) + 4 * h5 + (r & 3)) * VS + l31;
 #pragma unroll
-                for (int d = 0; d < DH / 32; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], p[tb][r], o[d], 0, 0, 0);
+                for (int w = 0; w < RW; ++w) l[w] += p[w][tb][r];
+#pragma unroll
+                for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                    for (int w = 0; w < RW; ++w) o[w][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[32 * d], p[w][tb][r], o[w][d], 0, 0, 0);
             }
     }
     __device__ static __forceinline__ bool finite_only(f32x4& x) {
@@ -402,86 +417,108 @@ __device__ __forceinline__ QFrag load_q(const PagedArgs& a, const T* row, int ch
     return q;
 }
 
-// One wave's 32 rows, a row on each lane (and on lane ^ 32, which holds the other half of the keys of a tile).
-template <typename T, int DH>
+// One wave's RW x 32 rows, row 32 i + (lane & 31) on two lanes (lane ^ 32 holds the other half of the keys of a tile).
+template <typename T, int DH, int RW>
 struct Rows {
     typedef Prod<T, DH> P_;
-    typename P_::QFrag q[P_::NQ];
-    f32x16 o[DH / 32];
-    float m, l, c, bias;          // running maximum (raw scores), sum, scale * log2e, slope in raw-score units
-    int limit, at;                // last key this row sees, its position
-    int first_limit, last_limit;  // the smallest and largest limit of the wave's rows
+    typename P_::QFrag q[RW][P_::NQ];
+    f32x16 o[RW][DH / 32];
+    float m[RW], l[RW], bias[RW], c;      // running maximum (raw scores), sum, slope in raw-score units; |scale| * log2e
+    int limit[RW], at[RW];                // last key the row sees, its position
+    int first_limit, last_limit;          // the smallest and largest limit of the wave's rows
 
-    // row: this lane's row of q (element pointer at its head), or NULL
-    __device__ __forceinline__ void begin(const PagedArgs& a, const T* row, int h5, float slope, int limit_, int at_) {
+    __device__ __forceinline__ void begin(const PagedArgs& a) {
         c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
-        bias = slope * LOG2E / c;
-        limit = limit_;
-        at = at_;
+        first_limit = 0x7FFFFFFF;
+        last_limit = -1;
+    }
+    // row: this lane's row i of q (element pointer at its head), or NULL
+    __device__ __forceinline__ void begin_row(const PagedArgs& a, int i, const T* row, int h5, float slope, int limit_, int at_) {
+        bias[i] = slope * LOG2E / c;
+        limit[i] = limit_;
+        at[i] = at_;
         int lo = row ? limit_ : 0x7FFFFFFF, hi = row ? limit_ : -1;
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) {
             lo = min(lo, __shfl_xor(lo, s, 64));
             hi = max(hi, __shfl_xor(hi, s, 64));
         }
-        first_limit = __builtin_amdgcn_readfirstlane(lo);
-        last_limit = __builtin_amdgcn_readfirstlane(hi);
-        m = NEG;
-        l = 0.f;
+        first_limit = min(first_limit, __builtin_amdgcn_readfirstlane(lo));
+        last_limit = max(last_limit, __builtin_amdgcn_readfirstlane(hi));
+        m[i] = NEG;
+        l[i] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < P_::NQ; ++ks) q[ks] = load_q<T, typename P_::QFrag>(a, row, P_::qchunk(ks, h5));
+        for (int ks = 0; ks < P_::NQ; ++ks) q[i][ks] = load_q<T, typename P_::QFrag>(a, row, P_::qchunk(ks, h5));
 #pragma unroll
         for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+            for (int r = 0; r < 16; ++r) o[i][d][r] = 0.f;
     }
     // NB blocks of 32 keys from j0 on; seen: the keys that are somewhere
     template <int NB, bool ALIBI>
     __device__ __forceinline__ void take(const P_& pr, const char* K, const char* V, int j0, unsigned long long seen, int h5) {
-        f32x16 s[NB];
-        const float lb = ALIBI ? bias * (float)(j0 + 4 * h5 - at) : 0.f;
+        f32x16 s[RW][NB];
 #pragma unroll
-        for (int tb = 0; tb < NB; ++tb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[tb][r] = ALIBI ? fmaf(bias, (float)(32 * tb + (r & 3) + 8 * (r >> 2)), lb) : 0.f;
-        pr.template scores<NB>(K, q, s);
-        const typename P_::VAhead va = pr.vread(V, 0, 0);
-        const unsigned long long all = NB == 2 ? ~0ull : 0xFFFFFFFFull;
-        if (seen != all || j0 + 32 * NB - 1 > first_limit) {          // uniform
-            const int dj = limit - j0 - 4 * h5;
-            const unsigned long long mine = seen >> (4 * h5);
+        for (int i = 0; i < RW; ++i) {
+            const float lb = ALIBI ? bias[i] * (float)(j0 + 4 * h5 - at[i]) : 0.f;
 #pragma unroll
             for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int kk = 32 * tb + (r & 3) + 8 * (r >> 2);
-                    if (kk > dj || !((mine >> kk) & 1)) s[tb][r] = -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r) s[i][tb][r] = ALIBI ? fmaf(bias[i], (float)(32 * tb + (r & 3) + 8 * (r >> 2)), lb) : 0.f;
         }
-        float mx = s[0][0];
+        pr.template scores<NB, RW>(K, q, s);
+        const typename P_::VAhead va = pr.vread(V, 0, 0);
+        const unsigned long long all = NB == 2 ? ~0ull : 0xFFFFFFFFull;
+        if (seen != all || j0 + 32 * NB - 1 > first_limit) {          // uniform
+            const unsigned long long mine = seen >> (4 * h5);
 #pragma unroll
-        for (int tb = 0; tb < NB; ++tb)
+            for (int i = 0; i < RW; ++i) {
+                const int dj = limit[i] - j0 - 4 * h5;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[tb][r]);
-        mx = half_swap_max(mx);
+                for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int kk = 32 * tb + (r & 3) + 8 * (r >> 2);
+                        if (kk > dj || !((mine >> kk) & 1)) s[i][tb][r] = -INFINITY;
+                    }
+            }
+        }
+        float mx[RW];
+        bool grown = false;
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            float x = s[i][0][0];
+#pragma unroll
+            for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x = fmaxf(x, s[i][tb][r]);
+            mx[i] = half_swap_max(x);
+            grown |= !((mx[i] - m[i]) * c <= RESCALE_LOG2);
+        }
         // the stale maximum stays while no row's grew by more than 2^8: weights are then at most 2^8, which fp32 sums and
         // bf16 weights hold with the same relative precision
-        if (!__all((mx - m) * c <= RESCALE_LOG2)) {
-            const float mn = fmaxf(m, mx);
-            const float alpha = fast_exp2((m - mn) * c);
-            m = mn;
-            l *= alpha;
+        if (__any(grown)) {
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d)
+            for (int i = 0; i < RW; ++i) {
+                const float mn = fmaxf(m[i], mx[i]);
+                const float alpha = fast_exp2((m[i] - mn) * c);
+                m[i] = mn;
+                l[i] *= alpha;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+                for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[i][d][r] *= alpha;
+            }
         }
-        const float mc = m * c;
 #pragma unroll
-        for (int tb = 0; tb < NB; ++tb)
+        for (int i = 0; i < RW; ++i) {
+            const float mc = m[i] * c;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[tb][r] = fast_exp2(fmaf(s[tb][r], c, -mc));
-        pr.template weigh<NB>(V, va, s, o, l);
+            for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][tb][r] = fast_exp2(fmaf(s[i][tb][r], c, -mc));
+        }
+        pr.template weigh<NB, RW>(V, va, s, o, l);
     }
     // Keys j0 .. j0+31, whose V values that are not finite were left out: rows that see such a key get NaN there.
     __device__ __forceinline__ void spoil(const PagedArgs& a, const int* own, int hk, int j0, int end, int h5) {
@@ -494,7 +531,10 @@ struct Rows {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int at_d = 32 * d + 8 * (r >> 2) + 4 * h5 + (r & 3);
-                    if (at_d < a.dh && j <= limit && !(fabsf(to_f32(v[at_d])) < INFINITY)) o[d][r] = __builtin_nanf("");
+                    const bool bad = at_d < a.dh && !(fabsf(to_f32(v[at_d])) < INFINITY);
+#pragma unroll
+                    for (int i = 0; i < RW; ++i)
+                        if (bad && j <= limit[i]) o[i][d][r] = __builtin_nanf("");
                 }
         }
     }
@@ -817,22 +857,26 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
     }
 }
 
-template <typename T, int DH, bool ALIBI>
+template <typename T, int DH, int RW, bool ALIBI>
 __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod<T, DH> P_;
     constexpr int TB = 2 * (P_::KB + P_::VB);                           // one 64-key buffer: K, then V
-    constexpr long TR = 32 * NW;
+    constexpr long TR = 32 * RW * NW;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
     const P_ pr(lane);
     int* odd = reinterpret_cast<int*>(smem + 2 * TB);                   // first and last key of the tiles with V values left out
     const int* own = a.table + (long)it.b * a.width;
     for (int rt = it.rt; rt * TR < (long)it.n * G; rt += it.rts) {
-        long t;
-        int h, limit, at;
-        const T* row = item_row<T>(a, it, rt * TR + 32 * w + l31, G, t, h, limit, at);
-        Rows<T, DH> rows;
-        rows.begin(a, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
+        Rows<T, DH, RW> rows;
+        rows.begin(a);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            long t;
+            int h, limit, at;
+            const T* row = item_row<T>(a, it, rt * TR + 32 * (RW * w + i) + l31, G, t, h, limit, at);
+            rows.begin_row(a, i, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
+        }
         // the range ends behind the last key any row of the workgroup sees; masked keys begin behind the first row's
         int end = it.k1, sure = it.k1;
         if (!it.prefix) {
@@ -891,8 +935,12 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             __syncthreads();
         }
         for (int j = odd[0]; j <= odd[1]; j += 32) rows.spoil(a, own, it.hk, j, end, h5);
-        const float den = half_swap_sum(rows.l);
-        if (row) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            long t;
+            int h, limit, at;
+            if (!item_row<T>(a, it, rt * TR + 32 * (RW * w + i) + l31, G, t, h, limit, at)) continue;
+            const float den = half_swap_sum(rows.l[i]);          // (both lanes of a row are here)
             const long orow = t * a.Hq + h;
             const long slot = (long)it.split * a.T * a.Hq + orow;
             const float inv = it.direct ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
@@ -904,12 +952,12 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
                     if (d0 >= a.dh) continue;
                     float x[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] = rows.o[d][4 * g + k] * inv;
+                    for (int k = 0; k < 4; ++k) x[k] = rows.o[i][d][4 * g + k] * inv;
                     if (it.direct) put4((T*)a.out + orow * a.dh + d0, x);
                     else put4(a.acc + slot * a.dh + d0, x);
                 }
             if (!it.direct && h5 == 0) {
-                a.ml[2 * slot] = rows.m * rows.c;
+                a.ml[2 * slot] = rows.m[i] * rows.c;
                 a.ml[2 * slot + 1] = den;
             }
         }
@@ -917,10 +965,10 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
     }
 }
 
-// BODY: 0 / 1 private with 16 / 32 rows, 2 shared
+// BODY: 0 / 1 private with 16 / 32 rows, 2 / 3 shared with 32 / 64 rows a wave
 template <typename T, int DH, int BODY>
 constexpr int body_smem() {
-    if (BODY == 2) return 4 * (Prod<T, DH>::KB + Prod<T, DH>::VB) + 16;
+    if (BODY >= 2) return 4 * (Prod<T, DH>::KB + Prod<T, DH>::VB) + 16;
     const int tiles = NW * (Prod16<T, DH>::KB + Prod16<T, DH>::VB), rows = BODY == 1 ? 32 : 16, join = NW * rows * (DH + 4 + 2) * 4;
     return tiles > join ? tiles : join;
 }
@@ -938,7 +986,7 @@ __device__ __forceinline__ void clear_rows(const PagedArgs& a, int wg) {
 // ALIBI: slopes (shared items; the private ones, which wait for memory, add a slope of 0)
 template <typename T, int DH, int BODY, bool ALIBI>
 __device__ __forceinline__ void run_item(const PagedArgs& a, const Item& it, char* smem) {
-    if constexpr (BODY == 2) shared_item<T, DH, ALIBI>(a, it, smem);
+    if constexpr (BODY >= 2) shared_item<T, DH, BODY - 1, ALIBI>(a, it, smem);
     else private_item<T, DH, BODY + 1>(a, it, smem);
 }
 // Prefix items first, then own items, in one launch: the former are bound by arithmetic, the latter by memory, and a CU holds
@@ -1090,18 +1138,21 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     p.rows_only = dh > 128;                            // a wave's sums, q and staged keys no longer fit its registers
     const long G = Hq / Hkv, rows = (long)max_rows * G;
     const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : 128;
-    auto body_of = [](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : 2; };
-    auto tile_rows = [](int body) { return body == 2 ? 32L * NW : 16L * (body + 1); };
+    // 64 rows a wave share the reads, the page look-ups and the staging of a tile (bf16 heads of 64: prefix items of 3840 rows
+    // and 16385 keys XXX us); with 128 sums a row more they would not fit two waves a SIMD
+    auto body_of = [&](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
+    auto tile_rows = [](int body) { return body >= 2 ? 32L * NW * (body - 1) : 16L * (body + 1); };
     // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
     // sequence whose rows fill a tile by themselves has nothing to gain.
     p.share = P > 0 && B > 1 && T * G < 128L * B;
     p.body_o = body_of(rows);
     p.body_p = p.share ? body_of(T * G) : p.body_o;
-    if (p.body_p == 1 || (p.body_o > p.body_p)) p.body_o = p.body_p;     // (instances: private items of 32 rows take 16, too)
+    if (p.body_p == 1 || p.body_o > p.body_p) p.body_o = p.body_p;       // (fewer instances: a body of more rows takes less)
+    if (p.body_p == 3 && p.body_o == 2) p.body_o = 3;
     const double row_us = T * Hq * (dh + 2.0) * 8.0 / 5.0e6;              // one part of every row, written and read
     const long key_bytes = 2L * dh * bytes;
     auto parts = [&](long base, long keys, int body, bool join, int& chunk) {
-        if (body == 2) {                               // compute: about 1.3 us for 64 keys of dh 128 against 256 rows
+        if (body >= 2) {                               // compute: about 1.3 us for 64 keys of dh 128 against 256 rows
             const double key = 0.01 * DH / 128 * (bytes == 4 ? 8 : 1) + 0.01;
             return parts_of(base, keys, 64, 512, 5.0, key, row_us, join, chunk);
         }
@@ -1135,25 +1186,35 @@ int launch_items(const PagedArgs& a, long items_p, long items_o, hipStream_t st)
     return MGX_OK;
 }
 
-template <typename T, int DH>
-int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
-    const long ip = p.share ? ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p : 0, io = (long)a.B * a.Hkv * p.rt_o * p.So;
-    int rc;
-    if (p.body_p < 2) rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
-    else if (a.slopes)
-        rc = p.body_o == 2   ? launch_items<T, DH, 2, 2, true>(a, ip, io, st)
-             : p.body_o == 1 ? launch_items<T, DH, 2, 1, true>(a, ip, io, st)
-                             : launch_items<T, DH, 2, 0, true>(a, ip, io, st);
-    else
-        rc = p.body_o == 2   ? launch_items<T, DH, 2, 2, false>(a, ip, io, st)
-             : p.body_o == 1 ? launch_items<T, DH, 2, 1, false>(a, ip, io, st)
-                             : launch_items<T, DH, 2, 0, false>(a, ip, io, st);
-    if (rc || (!p.share && p.So == 1)) return rc;
+template <typename T, int DH, int BODY_P, bool ALIBI>
+int launch_wide(const PagedArgs& a, int body_o, long items_p, long items_o, hipStream_t st) {
+    return body_o >= 2   ? launch_items<T, DH, BODY_P, BODY_P, ALIBI>(a, items_p, items_o, st)
+           : body_o == 1 ? launch_items<T, DH, BODY_P, 1, ALIBI>(a, items_p, items_o, st)
+                         : launch_items<T, DH, BODY_P, 0, ALIBI>(a, items_p, items_o, st);
+}
+
+template <typename T>
+int launch_join(const PagedArgs& a, hipStream_t st) {
     const long blocks = ceil_div(a.T * a.Hq * (a.dh / 4), 256);
     MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
     hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
     MGX_CHECK_LAUNCH("paged_join");
     return MGX_OK;
+}
+
+template <typename T, int DH>
+int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
+    const long ip = p.share ? ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p : 0, io = (long)a.B * a.Hkv * p.rt_o * p.So;
+    int rc;
+    if constexpr (sizeof(T) == 2 && DH == 64) {
+        if (p.body_p == 3) {
+            rc = a.slopes ? launch_wide<T, DH, 3, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, 3, false>(a, p.body_o, ip, io, st);
+            return rc || (!p.share && p.So == 1) ? rc : launch_join<T>(a, st);
+        }
+    }
+    if (p.body_p == 2) rc = a.slopes ? launch_wide<T, DH, 2, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, 2, false>(a, p.body_o, ip, io, st);
+    else rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
+    return rc || (!p.share && p.So == 1) ? rc : launch_join<T>(a, st);
 }
 
 }  // namespace
