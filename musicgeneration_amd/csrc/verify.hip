@@ -19,11 +19,11 @@ template <typename T>
 struct Row {
     const T *p, *q;          // q NULL: nothing is taken off but the one-hot at `lost`
     long long lost;          // class whose weight is dropped, -1: none
-    __device__ __forceinline__ double clean(float x) const { return x > 0.f && x < INFINITY ? (double)x : 0.0; }
+    // positive and finite: classes 7 and 8 (denormal, normal) of v_cmp_class_f32
+    __device__ __forceinline__ double clean(float x) const { return __builtin_amdgcn_classf(x, 0x180) ? (double)x : 0.0; }
     __device__ __forceinline__ double weight(float pv, float qv, long c) const {
-        if (c == lost) return 0.0;
-        const double d = clean(pv) - clean(qv);
-        return d > 0.0 ? d : 0.0;
+        const double d = fmax(clean(pv) - clean(qv), 0.0);
+        return c == lost ? 0.0 : d;
     }
     __device__ __forceinline__ double at(long c) const { return weight(to_f32(p[c]), q ? to_f32(q[c]) : 0.f, c); }
 };
@@ -37,21 +37,25 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // this wave's sum over classes [c0, c1): U independent loads in flight per lane
 template <typename T>
 __device__ __forceinline__ double slice_sum(const Row<T>& row, long c0, long c1, int lane) {
-    constexpr int U = 8;
-    double s = 0.0;
+    constexpr int U = 16;
+    double s[2] = {0.0, 0.0};
     long c = c0 + lane;
     for (; c + 64 * (U - 1) < c1; c += 64 * U) {
         float pv[U], qv[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             pv[k] = to_f32(row.p[c + 64 * k]);
-            qv[k] = row.q ? to_f32(row.q[c + 64 * k]) : 0.f;
+            qv[k] = 0.f;
+        }
+        if (row.q) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) qv[k] = to_f32(row.q[c + 64 * k]);
         }
 #pragma unroll
-        for (int k = 0; k < U; ++k) s += row.weight(pv[k], qv[k], c + 64 * k);
+        for (int k = 0; k < U; ++k) s[k & 1] += row.weight(pv[k], qv[k], c + 64 * k);
     }
-    for (; c < c1; c += 64) s += row.at(c);
-    return wave_sum64(s);
+    for (; c < c1; c += 64) s[0] += row.at(c);
+    return wave_sum64(s[0] + s[1]);
 }
 
 // The slice of the NW sums whose running total passes `target` (the last one with weight if none does), and the total
