@@ -427,24 +427,12 @@ struct Rows {
     int limit[RW], at[RW];                // last key the row sees, its position
     int first_limit, last_limit;          // the smallest and largest limit of the wave's rows
 
-    __device__ __forceinline__ void begin(const PagedArgs& a) {
-        c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
-        first_limit = 0x7FFFFFFF;
-        last_limit = -1;
-    }
+    __device__ __forceinline__ void begin(const PagedArgs& a) { c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f); }
     // row: this lane's row i of q (element pointer at its head), or NULL
     __device__ __forceinline__ void begin_row(const PagedArgs& a, int i, const T* row, int h5, float slope, int limit_, int at_) {
         bias[i] = slope * LOG2E / c;
         limit[i] = limit_;
         at[i] = at_;
-        int lo = row ? limit_ : 0x7FFFFFFF, hi = row ? limit_ : -1;
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
-            lo = min(lo, __shfl_xor(lo, s, 64));
-            hi = max(hi, __shfl_xor(hi, s, 64));
-        }
-        first_limit = min(first_limit, __builtin_amdgcn_readfirstlane(lo));
-        last_limit = max(last_limit, __builtin_amdgcn_readfirstlane(hi));
         m[i] = NEG;
         l[i] = 0.f;
 #pragma unroll
@@ -559,23 +547,11 @@ struct Rows16 {
     float m[RT], l[RT], bias[RT], c;
     int limit[RT], at[RT], first_limit, last_limit;
 
-    __device__ __forceinline__ void begin(const PagedArgs& a) {
-        c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);
-        first_limit = 0x7FFFFFFF;
-        last_limit = -1;
-    }
+    __device__ __forceinline__ void begin(const PagedArgs& a) { c = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f); }
     __device__ __forceinline__ void begin_row(const PagedArgs& a, int rt, const T* row, int g, float slope, int limit_, int at_) {
         bias[rt] = slope * LOG2E / c;
         limit[rt] = limit_;
         at[rt] = at_;
-        int lo = row ? limit_ : 0x7FFFFFFF, hi = row ? limit_ : -1;
-#pragma unroll
-        for (int s = 8; s > 0; s >>= 1) {
-            lo = min(lo, __shfl_xor(lo, s, 64));
-            hi = max(hi, __shfl_xor(hi, s, 64));
-        }
-        first_limit = min(first_limit, __builtin_amdgcn_readfirstlane(lo));
-        last_limit = max(last_limit, __builtin_amdgcn_readfirstlane(hi));
         m[rt] = NEG;
         l[rt] = 0.f;
 #pragma unroll
@@ -680,28 +656,34 @@ __device__ __forceinline__ void put4(T* p, const float* x) {
 struct Item {
     bool prefix, direct;         // prefix: rows of the whole batch, prefix keys; direct: the output itself, nothing to join
     int b, hk, rt, rts, split;   // row tile and tiles in the grid; split: slot among the parts that are joined
-    int k0, k1, n, own;          // key range, rows of the sequence, own keys
+    int k0, k1, n, first;        // key range, rows of the sequence, position of its first new row
     long row0;                   // first row (of q) of the sequence
 };
+
+// a length as the device holds it, kept where sums with it do not overflow (longer tables are refused)
+__device__ __forceinline__ int sane(int len) { return min(max(len, -(1 << 29)), 1 << 30); }
 
 __device__ __forceinline__ bool own_item(const PagedArgs& a, int id, Item& it) {
     it.prefix = false;
     it.rts = a.rt_o;
-    it.split = id % a.So;
-    int rest = id / a.So;
-    it.hk = rest % a.Hkv;
-    rest /= a.Hkv;
-    it.rt = rest % a.rt_o;
-    it.b = rest / a.rt_o;
+    const unsigned per_head = a.So, per_tile = per_head * a.Hkv, per_seq = per_tile * a.rt_o;
+    unsigned rest = id;
+    it.b = rest / per_seq;
+    rest -= it.b * per_seq;
+    it.rt = a.rt_o == 1 ? 0 : rest / per_tile;
+    rest -= it.rt * per_tile;
+    it.hk = per_head == 1 ? rest : rest / per_head;
+    it.split = rest - it.hk * per_head;
     it.row0 = (long)it.b * a.R;
     it.n = a.R;
     if (a.cu) {                                   // (offsets that are none stay inside the rows)
         it.row0 = min(max((long)a.cu[it.b], 0L), a.T);
         it.n = (int)(min(max((long)a.cu[it.b + 1], it.row0), a.T) - it.row0);
     }
-    it.own = min(max(a.lens[it.b], 0), a.width * a.page);
+    const int last = sane(a.lens[it.b]);
+    it.first = a.P + last - it.n;
     it.direct = !a.share && a.So == 1;
-    const int base = a.share ? a.P : 0, end = a.P + it.own;
+    const int base = a.share ? a.P : 0, end = a.P + min(max(last, 0), a.width * a.page);
     // ranges of chunk_o keys, the last one open: it takes what a longer sequence than announced has left
     it.k0 = base + it.split * a.chunk_o;
     it.k1 = it.split == a.So - 1 ? end : min(end, it.k0 + a.chunk_o);
@@ -725,28 +707,37 @@ __device__ __forceinline__ void prefix_item(const PagedArgs& a, int id, Item& it
     it.b = 0;
     it.row0 = 0;
     it.n = (int)a.T;
-    it.own = 0;
+    it.first = a.P;
     it.k0 = it.split * a.chunk_p;
     it.k1 = min(a.P, it.k0 + a.chunk_p);
 }
 
 // this lane's row of an item: its row of q (NULL: none), head, last key it sees, position
 template <typename T>
-__device__ __forceinline__ const T* item_row(const PagedArgs& a, const Item& it, long rho, int G, long& t, int& h, int& limit, int& at) {
-    t = it.row0 + rho / G;
-    h = it.hk * G + (int)(rho % G);
+__device__ __forceinline__ const T* item_row(const PagedArgs& a, const Item& it, int rho, int G, long& t, int& h, int& limit, int& at) {
+    const int r = (unsigned)rho / (unsigned)G;
+    t = it.row0 + r;
+    h = it.hk * G + rho - r * G;
     limit = at = a.P - 1;
-    if (rho >= (long)it.n * G || t >= a.T) return nullptr;
-    if (it.prefix) {
-        if (a.slopes) {
-            int b, r, n;
-            if (find_row(a, t, b, r, n)) at = a.P + a.lens[b] - n + r;
-        }
-    } else {
-        at = a.P + a.lens[it.b] - it.n + (int)(rho / G);
+    if (rho >= it.n * G || t >= a.T) return nullptr;
+    if (!it.prefix) {
+        at = it.first + r;
         limit = max(at, a.P - 1);
+    } else if (a.slopes) {
+        int b, rb, n;
+        if (find_row(a, t, b, rb, n)) at = a.P + sane(a.lens[b]) - n + rb;
     }
     return (const T*)a.q + t * a.qs + (long)h * a.dh;
+}
+// the smallest and largest last key of rows rho0 .. rho0 + rows - 1 of an item (limits ascend with the row)
+__device__ __forceinline__ void item_limits(const PagedArgs& a, const Item& it, int rho0, int rows, int G, int& lo, int& hi) {
+    const int total = it.n * G;
+    lo = hi = a.P - 1;
+    if (rho0 >= total) lo = 0x7FFFFFFF, hi = -1;
+    else if (!it.prefix) {
+        lo = max(it.first + (int)((unsigned)rho0 / (unsigned)G), a.P - 1);
+        hi = max(it.first + (int)((unsigned)(min(rho0 + rows, total) - 1) / (unsigned)G), a.P - 1);
+    }
 }
 
 template <typename T, int DH, int RT>
@@ -759,14 +750,15 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
     char* K = smem + w * (P_::KB + P_::VB);
     char* V = K + P_::KB;
     const int* own = a.table + (long)it.b * a.width;
-    for (int rt = it.rt; (long)rt * TR < (long)it.n * G; rt += it.rts) {
+    for (int rt = it.rt; rt * TR < it.n * G; rt += it.rts) {
         Rows16<T, DH, RT> rows;
         rows.begin(a);
+        item_limits(a, it, rt * TR, TR, G, rows.first_limit, rows.last_limit);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             long t;
             int h, limit, at;
-            const T* row = item_row<T>(a, it, rt * (long)TR + 16 * i + l15, G, t, h, limit, at);
+            const T* row = item_row<T>(a, it, rt * TR + 16 * i + l15, G, t, h, limit, at);
             rows.begin_row(a, i, row, g, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
         }
         const int end = min(it.k1, rows.last_limit + 1);
@@ -805,7 +797,7 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         constexpr int LD = DH + 4;
         float* part = reinterpret_cast<float*>(smem);                   // [NW][TR][LD]
         float* stat = part + NW * TR * LD;                              // [NW][TR][2]
-        const int nr = (int)min((long)TR, (long)it.n * G - rt * (long)TR);
+        const int nr = min(TR, it.n * G - rt * TR);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -825,7 +817,8 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         const int quads = a.dh / 4;
         for (int e = tid; e < nr * quads; e += 64 * NW) {
             const int rr = e / quads, d0 = 4 * (e - rr * quads);
-            const long rho = rt * (long)TR + rr, tt = it.row0 + rho / G;
+            const int rho = rt * TR + rr, r = (unsigned)rho / (unsigned)G;
+            const long tt = it.row0 + r;
             if (tt >= a.T) continue;
             float mm = stat[rr * 2], x[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
 #pragma unroll
@@ -838,7 +831,7 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
 #pragma unroll
                 for (int k = 0; k < 4; ++k) x[k] = fmaf(p[k], f, x[k]);
             }
-            const long orow = tt * a.Hq + it.hk * G + rho % G;
+            const long orow = tt * a.Hq + it.hk * G + rho - r * G;
             if (it.direct) {
                 const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
@@ -861,15 +854,16 @@ template <typename T, int DH, int RW, bool ALIBI>
 __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod<T, DH> P_;
     constexpr int TB = 2 * (P_::KB + P_::VB);                           // one 64-key buffer: K, then V
-    constexpr long TR = 32 * RW * NW;
+    constexpr int TR = 32 * RW * NW;
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h5 = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
     const P_ pr(lane);
     int* odd = reinterpret_cast<int*>(smem + 2 * TB);                   // first and last key of the tiles with V values left out
     const int* own = a.table + (long)it.b * a.width;
-    for (int rt = it.rt; rt * TR < (long)it.n * G; rt += it.rts) {
+    for (int rt = it.rt; rt * TR < it.n * G; rt += it.rts) {
         Rows<T, DH, RW> rows;
         rows.begin(a);
+        item_limits(a, it, rt * TR + 32 * RW * w, 32 * RW, G, rows.first_limit, rows.last_limit);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
             long t;
@@ -878,13 +872,10 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
             rows.begin_row(a, i, row, h5, a.slopes && row ? a.slopes[h] : 0.f, limit, at);
         }
         // the range ends behind the last key any row of the workgroup sees; masked keys begin behind the first row's
-        int end = it.k1, sure = it.k1;
-        if (!it.prefix) {
-            const long lastr = min((long)it.n * G, rt * TR + TR) - 1;
-            const int p0 = a.P + a.lens[it.b] - it.n;
-            end = min(end, max(p0 + (int)(lastr / G), a.P - 1) + 1);
-            sure = max(p0 + (int)(rt * TR / G), a.P - 1) + 1;
-        }
+        int sure, end;
+        item_limits(a, it, rt * TR, TR, G, sure, end);
+        end = min(it.k1, end + 1);
+        sure = it.prefix ? it.k1 : sure + 1;
         const int ntiles = end > it.k0 ? (end - it.k0 + 63) / 64 : 0;
         if (tid == 0) odd[0] = 0x7FFFFFFF, odd[1] = -1;
         Stage<P_, T, DH, 64, NW> st(lane, w);
@@ -1010,29 +1001,49 @@ __global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void page
     }
 }
 
-// the parts of every row joined: 4 values a thread
+// The parts of every row joined: 4 values a thread, 2^lq threads a row; where rows are few and parts many, L threads take
+// every L-th part and are joined through LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
-    const int quads = a.dh / 4;
-    const long e = (long)blockIdx.x * 256 + threadIdx.x, row = e / quads;
-    if (row >= a.T * a.Hq) return;
-    const int d0 = 4 * (int)(e - row * quads);
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a, int lq, int L) {
+    __shared__ float part[256][6];
+    const int tid = threadIdx.x, q = tid & ((1 << lq) - 1), i = (tid >> lq) & (L - 1), rows = 256 >> lq;      // L, rows: powers of two
+    const long row = (long)blockIdx.x * (rows / L) + (tid >> lq) / L;
+    const int d0 = 4 * q;
     int b, r, n;
-    if (!find_row(a, row / a.Hq, b, r, n)) return;                      // (cleared by the item launch)
     float x[4] = {0.f, 0.f, 0.f, 0.f}, mm = NEG, den = 0.f;
-    const int own = min(max(a.lens[b], 0), a.width * a.page), parts = (a.share ? a.Sp : 0) + own_parts(a, own);
-    const long step = a.T * a.Hq;
+    const bool real = row < a.T * a.Hq && d0 < a.dh && find_row(a, row / a.Hq, b, r, n);      // (others are cleared by the item launch)
+    if (real) {
+        const int own = min(max(a.lens[b], 0), a.width * a.page), parts = (a.share ? a.Sp : 0) + own_parts(a, own);
+        const long step = a.T * a.Hq;
 #pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
-        const long slot = s * step + row;
-        const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
-        const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
-        const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
-        mm = mn;
-        den = den * f0 + l * f1;
+        for (int s = i; s < parts; s += L) {
+            const long slot = s * step + row;
+            const float m = a.ml[2 * slot], l = a.ml[2 * slot + 1];
+            const f32x4 p = *reinterpret_cast<const f32x4*>(a.acc + slot * a.dh + d0);
+            const float mn = fmaxf(mm, m), f0 = fast_exp2(mm - mn), f1 = fast_exp2(m - mn);
+            mm = mn;
+            den = den * f0 + l * f1;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
+            for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + p[k] * f1;
+        }
     }
+    if (L > 1) {
+        part[tid][0] = mm;
+        part[tid][1] = den;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[tid][2 + k] = x[k];
+        __syncthreads();
+        if (!real || i > 0) return;
+        for (int o = 1; o < L; ++o) {
+            const float* y = part[tid + (o << lq)];
+            const float mn = fmaxf(mm, y[0]), f0 = fast_exp2(mm - mn), f1 = fast_exp2(y[0] - mn);
+            mm = mn;
+            den = den * f0 + y[1] * f1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = x[k] * f0 + y[2 + k] * f1;
+        }
+    }
+    if (!real) return;
     const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] *= inv;
@@ -1117,17 +1128,21 @@ struct Plan {
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// Parts of a key range: `base` items of `keys` keys each, of which `slots` workgroups run at once.  A part costs `fix` us of
-// beginning and end and `key` us a key; the parts' sums are written and read again (`row_us` us for all rows of a part);
-// `join`: one part alone would need neither that nor the join launch (4 us).  The cheapest of 1..64.
-inline int parts_of(long base, long keys, long unit, int slots, double fix, double key, double row_us, bool join, int& chunk) {
+// Into how many parts (1..64) a key range of `keys` keys goes, for `base` items of which `slots` workgroups run at once.
+// A part costs 5 us of beginning and end and `key` us a key where the chip is full (`solo` us where it is not); `beside` us
+// of other work share the launch.  The time is that of the rounds of parts or of all work spread evenly, whichever is more;
+// `row_us` us for writing and reading one part of all rows; the join launch, where one part alone would not need it.
+inline int parts_of(long base, long keys, long unit, int slots, double key, double solo, double beside, double row_us, bool join,
+                    int& chunk) {
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 64; ++s) {
         const long c = ceil_div(ceil_div(keys, s), unit) * unit, n = ceil_div(keys, c);
         if (n != s) continue;
-        const long rounds = ceil_div(base * s, slots);
-        const double cost = rounds * (fix + c * key) + (s > 1 && join ? 4.0 : 0.0) + (s > 1 || !join ? s : 0) * row_us;
+        const long rounds = base * s / slots, rest = base * s % slots;
+        const double items = rounds * (5.0 + c * key) + (rest ? 5.0 + c * (rest * 2 <= slots ? solo : key) : 0.0);
+        const double even = (double)base * s / slots * (5.0 + c * key) + beside;
+        const double cost = (items > even ? items : even) + (s > 1 || !join ? s * row_us : 0.0) + (s > 1 && join ? 4.0 : 0.0);
         if (cost < least) least = cost, best = s, chunk = (int)c;
     }
     return best;
@@ -1139,7 +1154,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     const long G = Hq / Hkv, rows = (long)max_rows * G;
     const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : 128;
     // 64 rows a wave share the reads, the page look-ups and the staging of a tile (bf16 heads of 64: prefix items of 3840 rows
-    // and 16385 keys XXX us); with 128 sums a row more they would not fit two waves a SIMD
+    // and 16385 keys: 129 -> 112 us); with 128 sums a row more they would not fit two waves a SIMD
     auto body_of = [&](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
     auto tile_rows = [](int body) { return body >= 2 ? 32L * NW * (body - 1) : 16L * (body + 1); };
     // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
@@ -1149,22 +1164,25 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     p.body_p = p.share ? body_of(T * G) : p.body_o;
     if (p.body_p == 1 || p.body_o > p.body_p) p.body_o = p.body_p;       // (fewer instances: a body of more rows takes less)
     if (p.body_p == 3 && p.body_o == 2) p.body_o = 3;
-    const double row_us = T * Hq * (dh + 2.0) * 8.0 / 5.0e6;              // one part of every row, written and read
-    const long key_bytes = 2L * dh * bytes;
-    auto parts = [&](long base, long keys, int body, bool join, int& chunk) {
-        if (body >= 2) {                               // compute: about 1.3 us for 64 keys of dh 128 against 256 rows
-            const double key = 0.01 * DH / 128 * (bytes == 4 ? 8 : 1) + 0.01;
-            return parts_of(base, keys, 64, 512, 5.0, key, row_us, join, chunk);
+    const double row_us = T * Hq * (dh + 2.0) * 8.0 / 4.2e6;
+    const double key_bytes = 2.0 * dh * bytes;
+    // Own lengths are taken to be half of the announced maximum on average.  A workgroup alone streams 25 bytes/ns, the chip
+    // 5 bytes/ps.  Shared items: us a key as measured with two workgroups a CU (128 rows of dh 128: 2.6 us for 64 keys);
+    // alone a workgroup takes 0.6 of that, beside own items 0.8.
+    const double own_us = 0.5 * B * Hkv * (double)max_len * key_bytes / 5.0e6;
+    auto parts = [&](long base, long keys, int body, bool join, double beside, int& chunk) {
+        if (body < 2) {
+            return parts_of(base, keys, 128, 512, 0.5 * key_bytes * 512 / 5.0e6, key_bytes / 25.0e3, beside, row_us, join, chunk);
         }
-        const int slots = 512;                         // two workgroups a CU: 25 bytes/ns each alone, 5 TB/s together
-        const double rate = 5.0e6 / (double)(base < slots ? (base > 200 ? base : 200) : slots);
-        return parts_of(base, keys, 128, slots, 4.0, key_bytes / rate, row_us, join, chunk);
+        const double key = bytes == 4 ? (DH == 64 ? 0.11 : 0.22) : body == 3 ? 0.047 : DH == 64 ? 0.028 : 0.04;
+        return parts_of(base, keys, 64, bytes == 4 && DH == 128 ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
+                        row_us, join, chunk);
     };
     p.rt_o = (int)ceil_div(rows, tile_rows(p.body_o));
-    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, !p.share, p.chunk_o);
+    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, !p.share, 0.0, p.chunk_o);
     if (p.share) {
         p.rt_p = (int)ceil_div(T * G, tile_rows(p.body_p));
-        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, false, p.chunk_p);
+        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, false, own_us, p.chunk_p);
     }
     return p;
 }
@@ -1195,9 +1213,14 @@ int launch_wide(const PagedArgs& a, int body_o, long items_p, long items_o, hipS
 
 template <typename T>
 int launch_join(const PagedArgs& a, hipStream_t st) {
-    const long blocks = ceil_div(a.T * a.Hq * (a.dh / 4), 256);
+    int lq = 0, L = 1;
+    while (4 << lq < a.dh) ++lq;
+    const long rows = a.T * a.Hq;
+    const int parts = (a.share ? a.Sp : 0) + a.So;
+    while ((rows << lq) * L < 65536 && (L << lq) < 256 && 2 * L <= parts) L *= 2;       // a wave on each SIMD
+    const long blocks = ceil_div(rows, (256 >> lq) / L);
     MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
-    hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a, lq, L);
     MGX_CHECK_LAUNCH("paged_join");
     return MGX_OK;
 }
@@ -1246,7 +1269,7 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
     MGX_REQUIRE(q_row_stride >= (long)Hq * dh && q_row_stride % N == 0, MGX_EINVAL, "mgx_paged_attn: row stride %ld", q_row_stride);
     MGX_REQUIRE((((uintptr_t)q | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out) & 15) == 0, MGX_EINVAL,
                 "mgx_paged_attn: tensors must be 16-byte aligned");
-    MGX_REQUIRE(Hq <= 65535, MGX_EUNSUPPORTED, "mgx_paged_attn: Hq=%d", Hq);
+    MGX_REQUIRE(Hq <= 65535 && T * Hq < (1L << 30), MGX_EUNSUPPORTED, "mgx_paged_attn: T=%ld rows of Hq=%d heads", T, Hq);
     const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
     MGX_REQUIRE(workspace || p.rows_only || (!p.share && p.So == 1), MGX_EINVAL, "mgx_paged_attn: no workspace");
     MGX_REQUIRE((long)n_pages * Hkv * page < 0xFFFFFFFFL, MGX_EUNSUPPORTED, "mgx_paged_attn: pool of more than 2^32 rows");

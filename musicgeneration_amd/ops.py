@@ -1458,6 +1458,8 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     T = out.numel() // (Hq * dh)
     if T == 0:
         return out
+    if T * Hq >= 2 ** 30:
+        raise ValueError(f"{name}: {T} rows of {Hq} heads")
     R = 0 if cu_rows is not None else q.shape[1]
     max_rows = R or min(T, T if max_rows is None else max_rows)
     max_len = page * width if max_len is None else min(max_len, page * width)
