@@ -10,6 +10,10 @@ own (SimpleAttention.forward, RelativeAttention.forward, Norm, the criteria) cal
     torch.ops.mgx.rel_attention(qkv, E, n_heads) -> out                 differentiable in qkv and E
     torch.ops.mgx.layer_norm(x, gamma, beta, eps) -> y                  differentiable in x, gamma, beta
     torch.ops.mgx.gemm_nt(a, bt, bias) -> c                             a @ bt^T + bias, differentiable in a, bt, bias
+    torch.ops.mgx.rotary(x, cos, sin, positions, layout, transposed) -> y    differentiable in x
+    torch.ops.mgx.paged_append(qkv, kcache!, vcache!, table, lens, ...) -> q   files k and v in place
+    torch.ops.mgx.paged_attention(q, kcache, vcache, table, lens, ...) -> out  serving, no gradient
+    torch.ops.mgx.verify_draft(target, tokens, uniforms, draft, counts) -> (tokens, accepted)
     torch.ops.mgx.alibi_attn_fwd / alibi_attn_bwd / gemm_tn / colsum    building blocks (no autograd formula)
 """
 from __future__ import annotations
@@ -221,3 +225,66 @@ def _gemm_backward(ctx, dc):
 
 
 gemm_nt.register_autograd(_gemm_backward, setup_context=_gemm_setup)
+
+
+# ---- rotary positions and the paged cache (ops.py) ----------------------------------------------------------------------
+@_lib.custom_op("mgx::rotary", mutates_args=())
+def rotary(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None, layout: str = "interleaved",
+           transposed: bool = False) -> Tensor:
+    half = ops._rotary_args(x, cos, sin, positions, layout, "rotary")
+    return ops._rotary(x, ops._dense_like(x), cos, sin, positions, half, 1 if transposed else 0)
+
+
+@rotary.register_fake
+def _(x, cos, sin, positions=None, layout="interleaved", transposed=False):
+    return x.new_empty(x.shape)
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, cos, sin, positions, ctx.layout, ctx.transposed = inputs
+    ctx.save_for_backward(cos, sin, positions)
+
+
+def _rotary_backward(ctx, dy):
+    cos, sin, positions = ctx.saved_tensors
+    dy = dy if dy.stride(-1) == 1 else dy.contiguous()
+    return torch.ops.mgx.rotary(dy, cos, sin, positions, ctx.layout, not ctx.transposed), None, None, None, None, None
+
+
+rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+@_lib.custom_op("mgx::paged_append", mutates_args=("kcache", "vcache"))
+def paged_append(qkv: Tensor, kcache: Tensor, vcache: Tensor, table: Tensor, lens: Tensor, n_heads: int,
+                 cos: Optional[Tensor] = None, sin: Optional[Tensor] = None, layout: str = "interleaved",
+                 cu_rows: Optional[Tensor] = None, offset: int = 0) -> Tensor:
+    q = ops.paged_append(qkv, kcache, vcache, table, lens, n_heads, cos, sin, layout, cu_rows, offset)
+    return q if cos is not None else q.clone(memory_format=torch.contiguous_format)     # (never a view of qkv)
+
+
+@paged_append.register_fake
+def _(qkv, kcache, vcache, table, lens, n_heads, cos=None, sin=None, layout="interleaved", cu_rows=None, offset=0):
+    return qkv.new_empty(*qkv.shape[:-1], n_heads, kcache.shape[3])
+
+
+@_lib.custom_op("mgx::paged_attention", mutates_args=())
+def paged_attention(q: Tensor, kcache: Tensor, vcache: Tensor, table: Tensor, lens: Tensor, slopes: Optional[Tensor] = None,
+                    cu_rows: Optional[Tensor] = None, max_rows: Optional[int] = None, max_len: Optional[int] = None,
+                    prefix: Optional[Tensor] = None, prefix_len: int = 0, scale: Optional[float] = None) -> Tensor:
+    return ops.paged_attn(q, kcache, vcache, table, lens, slopes, cu_rows, max_rows, max_len, prefix, prefix_len, scale)
+
+
+@paged_attention.register_fake
+def _(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_rows=None, max_len=None, prefix=None, prefix_len=0, scale=None):
+    return q.new_empty(q.shape)
+
+
+@_lib.custom_op("mgx::verify_draft", mutates_args=())
+def verify_draft(target: Tensor, tokens: Tensor, uniforms: Tensor, draft: Optional[Tensor] = None,
+                 counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    return ops.verify_draft(target, tokens, uniforms, draft, counts)
+
+
+@verify_draft.register_fake
+def _(target, tokens, uniforms, draft=None, counts=None):
+    return tokens.new_empty(tokens.shape[0], target.shape[1]), tokens.new_empty(tokens.shape[0], dtype=torch.int32)
