@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, 
     const int h = blockIdx.y, hk = h / (a.Hq / a.Hkv);
     int b, r, n;
     const bool real = find_row(a, t, b, r, n);
-    const int own = real ? min(max(a.lens[b] - n + r + 1, 0), a.width * a.page) : 0;
+    const int own = real ? min(max(sane(a.lens[b]) - n + r + 1, 0), a.width * a.page) : 0;
     const int keys = real ? a.P + own : 0, i = keys - 1;
     const int sub = lane / lpr, ch = lane % lpr, rpl = 64 / lpr;
     const bool has = ch * N < a.dh;

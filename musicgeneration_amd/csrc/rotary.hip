@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
         r = (int)(t - (long)b * a.R);
         n = a.R;
     }
-    const int index = a.lens[b] - n + r;
+    const int index = min(max(a.lens[b], -(1 << 29)), 1 << 30) - n + r;      // (no sum of an absurd length overflows)
     T* kdst = nullptr;
     T* vdst = nullptr;
     if (real && index >= 0 && index / a.page < a.width) {
@@ -323,11 +323,11 @@ extern "C" int mgx_paged_append(const void* qkv, void* q_out, void* kcache, void
     MGX_REQUIRE(qkv && kcache && vcache && table && lens, MGX_EINVAL, "mgx_paged_append: null pointer");
     MGX_REQUIRE((cos_tab != nullptr) == (sin_tab != nullptr) && (!cos_tab || q_out), MGX_EINVAL,
                 "mgx_paged_append: cos, sin and q_out go together");
-    MGX_REQUIRE(T > 0 && T < (1L << 31) && B > 0 && Hq > 0 && Hkv > 0 && dh > 0 && page > 0 && n_pages > 0 && width > 0,
+    MGX_REQUIRE(T > 0 && T < (1L << 30) && B > 0 && Hq > 0 && Hkv > 0 && dh > 0 && page > 0 && n_pages > 0 && width > 0,
                 MGX_EINVAL, "mgx_paged_append: T=%ld B=%d Hq=%d Hkv=%d dh=%d page=%d pages=%d width=%d", T, B, Hq, Hkv, dh,
                 page, n_pages, width);
     MGX_REQUIRE(cu_rows || (R > 0 && (long)B * R == T), MGX_EINVAL, "mgx_paged_append: B=%d x R=%d rows, got %ld", B, R, T);
-    MGX_REQUIRE((long)page * width < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_append: table beyond 2^31 keys");
+    MGX_REQUIRE((long)page * width < (1L << 30), MGX_EUNSUPPORTED, "mgx_paged_append: table beyond 2^30 keys");
     MGX_REQUIRE(offset >= 0, MGX_EINVAL, "mgx_paged_append: offset %d", offset);
     MGX_REQUIRE(dtype == MGX_F32 || dtype == MGX_BF16, MGX_EINVAL, "mgx_paged_append: bad dtype %d", dtype);
     const int N = dtype == MGX_F32 ? 4 : 8;

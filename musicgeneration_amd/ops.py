@@ -1465,6 +1465,7 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     max_len = page * width if max_len is None else min(max_len, page * width)
     if max_rows < 1 or max_len < 0:
         raise ValueError(f"{name}: max_rows {max_rows}, max_len {max_len}")
+    max_len = max(max_len, 1)
     # one row stride over the whole batch, heads dense inside a row
     st = q.stride()
     if cu_rows is None:
@@ -1482,7 +1483,7 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     check(_on(q.device, lambda s: lib.mgx_paged_attn(
         q.data_ptr(), row, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows), _p(slopes),
         _p(prefix) if prefix_len else None, out.data_ptr(), _p(ws), T, B, R, Hq, Hkv, dh, page, n_pages, width, prefix_len,
-        max_rows, max(max_len, 1), scale, dt, s)), "mgx_paged_attn")
+        max_rows, max_len, scale, dt, s)), "mgx_paged_attn")
     return out
 
 

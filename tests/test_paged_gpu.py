@@ -180,6 +180,57 @@ def test_attn_replays_in_two_graphs_with_other_lengths():
             assert_attended(out, want, bound)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("page", [7, 48])
+def test_attn_one_sequence_and_pages_of_any_size(dtype, page):
+    """Nothing to share with a batch of one: prefix and own keys meet inside a tile.  The hints' smallest values."""
+    for R, n, P in ((1, 1, 1), (3, 90, 50), (40, 40, 129), (2, 300, 0)):
+        k, v, table, prefix, g = _pool([n], 2, page, 64, dtype, P, seed=page + n)
+        q = torch.randn(1, R, 4, 64, generator=g).to(dtype)
+        _attend_both(q, k, v, table, [n], torch.tensor([1.0, 0.25, 0.0, 0.01]), prefix=prefix, P=P)
+        _attend_both(q, k, v, table, [n], prefix=prefix, P=P, max_len=0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dh", [64, 136])
+def test_attn_lengths_that_no_table_holds(dtype, dh):
+    """Lengths beyond the table and below zero: keys end where the table does, and begin at the first."""
+    k, v, table, prefix, g = _pool([48, 48, 48, 48], 2, 16, dh, dtype, 20, seed=dh)
+    table = table[:, :3].contiguous()
+    q = torch.randn(4, 2, 4, dh, generator=g).to(dtype)
+    for lens in ([48, 49, 50, 1000], [0, 1, -1, -50], [2 ** 31 - 1, -2 ** 31, 48, 47]):
+        _attend_both(q, k, v, table, lens, prefix=prefix, P=20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_append_beyond_the_table_files_nothing(dtype):
+    from musicgeneration_amd import ops
+    k, v, table, _, g = _pool([48, 48, 48, 48], 2, 16, 64, dtype, seed=4)
+    table = table[:, :3].contiguous().cuda()
+    qkv = torch.randn(4, 3, 6 * 64, generator=g).to(dtype).cuda()
+    kc, vc = k.cuda(), v.cuda()
+    ops.paged_append(qkv, kc, vc, table, torch.tensor([51, 2 ** 31 - 1, -2 ** 31, 0], dtype=torch.int32).cuda(), 2)
+    assert torch.equal(torch.nan_to_num(kc), torch.nan_to_num(k.cuda())) and torch.equal(torch.nan_to_num(vc), torch.nan_to_num(v.cuda()))
+
+
+def test_pool_past_32_bits():
+    """A pool of 6.4 GB a cache: pages at its far end serve as those of a small pool do, bit for bit."""
+    from musicgeneration_amd import ops
+    n, Hkv, page, dh = 48000, 4, 128, 128
+    cos, sin = ops.rope_tables(300, dh)
+    qkv = torch.randn(2, 200, (8 + 2 * Hkv) * dh, device="cuda").bfloat16()
+    lens = torch.tensor([200, 260], dtype=torch.int32).cuda()
+    outs = []
+    for pages, first in ((n, n - 6), (6, 0)):
+        kc, vc = (torch.empty(pages, Hkv, page, dh, dtype=BF16, device="cuda") for _ in range(2))
+        kc[first:].zero_(), vc[first:].zero_()
+        table = torch.arange(first, first + 6, dtype=torch.int32).view(2, 3).cuda()
+        q = ops.paged_append(qkv, kc, vc, table, lens, 8, cos, sin)
+        outs.append((ops.paged_attn(q, kc, vc, table, lens), ops.paged_attn(q[:, :1], kc, vc, table, lens), kc[first:].clone(), vc[first:].clone()))
+        del kc, vc
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and outs[0][2].any()
+
+
 # ---- paged_append -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("layout", ["interleaved", "half", None])
