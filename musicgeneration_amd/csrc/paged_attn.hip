@@ -740,10 +740,10 @@ __device__ __forceinline__ void item_limits(const PagedArgs& a, const Item& it, 
     }
 }
 
-template <typename T, int DH, int RT>
+template <typename T, int DH, int RT, int NWP>
 __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it, char* smem) {
     typedef Prod16<T, DH> P_;
-    constexpr int TR = 16 * RT, STEP = 32 * NW;
+    constexpr int TR = 16 * RT, STEP = 32 * NWP;
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4, l31 = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.Hq / a.Hkv;
     const P_ pr(lane);
@@ -795,8 +795,8 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         for (j = odd_first; j <= odd_last; j += STEP) rows.spoil(a, own, it.hk, j, end, g);
         // join the waves: sums relative to each wave's maximum, through LDS (over the tiles)
         constexpr int LD = DH + 4;
-        float* part = reinterpret_cast<float*>(smem);                   // [NW][TR][LD]
-        float* stat = part + NW * TR * LD;                              // [NW][TR][2]
+        float* part = reinterpret_cast<float*>(smem);                   // [NWP][TR][LD]
+        float* stat = part + NWP * TR * LD;                             // [NWP][TR][2]
         const int nr = min(TR, it.n * G - rt * TR);
         __syncthreads();
 #pragma unroll
@@ -815,16 +815,16 @@ __device__ __forceinline__ void private_item(const PagedArgs& a, const Item& it,
         }
         __syncthreads();
         const int quads = a.dh / 4;
-        for (int e = tid; e < nr * quads; e += 64 * NW) {
+        for (int e = tid; e < nr * quads; e += 64 * NWP) {
             const int rr = e / quads, d0 = 4 * (e - rr * quads);
             const int rho = rt * TR + rr, r = (unsigned)rho / (unsigned)G;
             const long tt = it.row0 + r;
             if (tt >= a.T) continue;
             float mm = stat[rr * 2], x[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
 #pragma unroll
-            for (int ww = 1; ww < NW; ++ww) mm = fmaxf(mm, stat[(ww * TR + rr) * 2]);
+            for (int ww = 1; ww < NWP; ++ww) mm = fmaxf(mm, stat[(ww * TR + rr) * 2]);
 #pragma unroll
-            for (int ww = 0; ww < NW; ++ww) {
+            for (int ww = 0; ww < NWP; ++ww) {
                 const float f = fast_exp2(stat[(ww * TR + rr) * 2] - mm);
                 den = fmaf(stat[(ww * TR + rr) * 2 + 1], f, den);
                 const f32x4 p = *reinterpret_cast<const f32x4*>(part + (ww * TR + rr) * LD + d0);
@@ -956,13 +956,22 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
     }
 }
 
-// BODY: 0 / 1 private with 16 / 32 rows, 2 / 3 shared with 32 / 64 rows a wave
+// BODY: 0 / 1 private with 16 / 32 rows, 2 / 3 shared with 32 / 64 rows a wave, 4 private with 16 rows and as many waves as
+// the LDS of a CU holds tiles for: few items of long sequences, each of which one workgroup takes without a join
+template <typename T, int DH, int BODY>
+constexpr int waves_of() {
+    if (BODY != 4) return NW;
+    const int fit = 136 * 1024 / (Prod16<T, DH>::KB + Prod16<T, DH>::VB);
+    return fit >= 16 ? 16 : fit >= 8 ? 8 : 4;
+}
 template <typename T, int DH, int BODY>
 constexpr int body_smem() {
-    if (BODY >= 2) return 4 * (Prod<T, DH>::KB + Prod<T, DH>::VB) + 16;
-    const int tiles = NW * (Prod16<T, DH>::KB + Prod16<T, DH>::VB), rows = BODY == 1 ? 32 : 16, join = NW * rows * (DH + 4 + 2) * 4;
+    if (BODY == 2 || BODY == 3) return 4 * (Prod<T, DH>::KB + Prod<T, DH>::VB) + 16;
+    const int nw = waves_of<T, DH, BODY>(), tiles = nw * (Prod16<T, DH>::KB + Prod16<T, DH>::VB);
+    const int join = nw * (BODY == 1 ? 32 : 16) * (DH + 4 + 2) * 4;
     return tiles > join ? tiles : join;
 }
+
 // rows of no sequence (ragged rows before the first or behind the last one): zeros, 64 workgroups
 constexpr int CLEARERS = 64;
 template <typename T>
@@ -977,13 +986,13 @@ __device__ __forceinline__ void clear_rows(const PagedArgs& a, int wg) {
 // ALIBI: slopes (shared items; the private ones, which wait for memory, add a slope of 0)
 template <typename T, int DH, int BODY, bool ALIBI>
 __device__ __forceinline__ void run_item(const PagedArgs& a, const Item& it, char* smem) {
-    if constexpr (BODY >= 2) shared_item<T, DH, BODY - 1, ALIBI>(a, it, smem);
-    else private_item<T, DH, BODY + 1>(a, it, smem);
+    if constexpr (BODY == 2 || BODY == 3) shared_item<T, DH, BODY - 1, ALIBI>(a, it, smem);
+    else private_item<T, DH, BODY == 1 ? 2 : 1, waves_of<T, DH, BODY>()>(a, it, smem);
 }
 // Prefix items first, then own items, in one launch: the former are bound by arithmetic, the latter by memory, and a CU holds
 // one of each.
 template <typename T, int DH, int BODY_P, int BODY_O, bool ALIBI>
-__global__ __launch_bounds__(64 * NW, (DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a, int items_p, int items) {
+__global__ __launch_bounds__((64 * waves_of<T, DH, BODY_O>()), (BODY_O == 4 ? waves_of<T, DH, BODY_O>() / 4 : DH * sizeof(T) <= 256 ? 2 : 1)) void paged_attn_kernel(const PagedArgs a, int items_p, int items) {
     extern __shared__ __attribute__((aligned(16))) char paged_smem[];
     Item it;
     const int id = blockIdx.x;
@@ -1133,9 +1142,9 @@ inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 // of other work share the launch.  The time is that of the rounds of parts or of all work spread evenly, whichever is more;
 // `row_us` us for writing and reading one part of all rows; the join launch, where one part alone would not need it.
 inline int parts_of(long base, long keys, long unit, int slots, double key, double solo, double beside, double row_us, bool join,
-                    int& chunk) {
+                    int& chunk, double& least) {
     int best = 1;
-    double least = 1e30;
+    least = 1e30;
     for (int s = 1; s <= 64; ++s) {
         const long c = ceil_div(ceil_div(keys, s), unit) * unit, n = ceil_div(keys, c);
         if (n != s) continue;
@@ -1156,33 +1165,53 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     // 64 rows a wave share the reads, the page look-ups and the staging of a tile (bf16 heads of 64: prefix items of 3840 rows
     // and 16385 keys: 129 -> 112 us); with 128 sums a row more they would not fit two waves a SIMD
     auto body_of = [&](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
-    auto tile_rows = [](int body) { return body >= 2 ? 32L * NW * (body - 1) : 16L * (body + 1); };
-    // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
-    // sequence whose rows fill a tile by themselves has nothing to gain.
-    p.share = P > 0 && B > 1 && T * G < 128L * B;
-    p.body_o = body_of(rows);
-    p.body_p = p.share ? body_of(T * G) : p.body_o;
-    if (p.body_p == 1 || p.body_o > p.body_p) p.body_o = p.body_p;       // (fewer instances: a body of more rows takes less)
-    if (p.body_p == 3 && p.body_o == 2) p.body_o = 3;
+    auto tile_rows = [](int body) { return body == 4 ? 16L : body >= 2 ? 32L * NW * (body - 1) : 16L * (body + 1); };
     const double row_us = T * Hq * (dh + 2.0) * 8.0 / 4.2e6;
     const double key_bytes = 2.0 * dh * bytes;
-    // Own lengths are taken to be half of the announced maximum on average.  A workgroup alone streams 25 bytes/ns, the chip
-    // 5 bytes/ps.  Shared items: us a key as measured with two workgroups a CU (128 rows of dh 128: 2.6 us for 64 keys);
-    // alone a workgroup takes 0.6 of that, beside own items 0.8.
-    const double own_us = 0.5 * B * Hkv * (double)max_len * key_bytes / 5.0e6;
-    auto parts = [&](long base, long keys, int body, bool join, double beside, int& chunk) {
-        if (body < 2) {
-            return parts_of(base, keys, 128, 512, 0.5 * key_bytes * 512 / 5.0e6, key_bytes / 25.0e3, beside, row_us, join, chunk);
+    // Own lengths are taken to be half of the announced maximum on average (a prefix read once for each sequence comes from
+    // L2, at twice the rate: the same half).  Four waves alone stream 25 bytes/ns (fp32, whose products take
+    // as long as its loads, 14), the chip 5 bytes/ps.  Shared items: us a key
+    // as measured with two workgroups a CU (128 rows of dh 128: 2.6 us for 64 keys); alone a workgroup takes 0.6 of that,
+    // beside own items 0.8.
+    auto parts = [&](long base, long keys, int body, bool join, double beside, int& chunk, double& us) {
+        if (body == 2 || body == 3) {
+            const double key = bytes == 4 ? (DH == 64 ? 0.11 : 0.22) : body == 3 ? 0.047 : DH == 64 ? 0.028 : 0.04;
+            return parts_of(base, keys, 64, bytes == 4 && DH == 128 ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
+                            row_us, join, chunk, us);
         }
-        const double key = bytes == 4 ? (DH == 64 ? 0.11 : 0.22) : body == 3 ? 0.047 : DH == 64 ? 0.028 : 0.04;
-        return parts_of(base, keys, 64, bytes == 4 && DH == 128 ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
-                        row_us, join, chunk);
+        const int groups = body == 4 ? 512 / (DH * bytes) : 1, slots = body == 4 ? 256 : 512;       // (waves_of) / 4
+        return parts_of(base, keys, 128 * groups, slots, 0.5 * key_bytes * slots / 5.0e6, (bytes == 4 ? 1.8 : 1.0) * key_bytes / (25.0e3 * groups), beside,
+                        row_us, join, chunk, us);
     };
-    p.rt_o = (int)ceil_div(rows, tile_rows(p.body_o));
-    p.So = parts((long)B * Hkv * p.rt_o, max_len + (p.share ? 0 : P), p.body_o, !p.share, 0.0, p.chunk_o);
-    if (p.share) {
-        p.rt_p = (int)ceil_div(T * G, tile_rows(p.body_p));
-        p.Sp = parts((long)Hkv * p.rt_p, P, p.body_p, false, own_us, p.chunk_p);
+    auto own = [&](Plan& o, int body, long keys, bool join, double& us) {
+        o.body_o = body;
+        o.rt_o = (int)ceil_div(rows, tile_rows(body));
+        const long full = T * G / tile_rows(body) + B, tiles = (long)B * o.rt_o < full ? (long)B * o.rt_o : full;      // ragged rows
+        o.So = parts(Hkv * tiles, keys, body, join, 0.0, o.chunk_o, us);
+    };
+    double us, wide_us = 1e30, apart_us = 1e30;
+    own(p, body_of(rows), (long)max_len + P, true, us);
+    p.body_p = p.body_o;
+    if (p.body_o == 0 && DH * bytes <= 256) {
+        Plan w = p;
+        own(w, 4, (long)max_len + P, true, wide_us);
+        if (wide_us < us) p = w, us = wide_us;
+    }
+    // Taking the prefix apart packs the rows of all sequences into its tiles and reads it once; it costs the join.  A
+    // sequence whose rows fill a tile by themselves has nothing to gain.
+    if (P > 0 && B > 1 && T * G < 128L * B) {
+        Plan s = p;
+        double own_us, prefix_us;
+        s.share = 1;
+        s.body_p = body_of(T * G);
+        int body = body_of(rows);
+        if (s.body_p == 1 || body > s.body_p) body = s.body_p;           // (fewer instances: a body of more rows takes less)
+        if (s.body_p == 3 && body == 2) body = 3;
+        own(s, body, max_len, false, own_us);
+        s.rt_p = (int)ceil_div(T * G, tile_rows(s.body_p));
+        s.Sp = parts((long)Hkv * s.rt_p, P, s.body_p, false, 0.5 * B * Hkv * (double)max_len * key_bytes / 5.0e6, s.chunk_p, prefix_us);
+        apart_us = (prefix_us > own_us ? prefix_us : own_us) + 4.0;
+        if (apart_us < us) p = s;
     }
     return p;
 }
@@ -1198,7 +1227,7 @@ int launch_items(const PagedArgs& a, long items_p, long items_o, hipStream_t st)
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, smem);
         MGX_REQUIRE(e == hipSuccess, MGX_ELAUNCH, "mgx_paged_attn: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O, ALIBI>), dim3((unsigned)grid), dim3(64 * NW), smem, st, a,
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, BODY_P, BODY_O, ALIBI>), dim3((unsigned)grid), dim3((64 * waves_of<T, DH, BODY_O>())), smem, st, a,
                        (int)items_p, (int)items);
     MGX_CHECK_LAUNCH("paged_attn");
     return MGX_OK;
@@ -1236,6 +1265,7 @@ int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
         }
     }
     if (p.body_p == 2) rc = a.slopes ? launch_wide<T, DH, 2, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, 2, false>(a, p.body_o, ip, io, st);
+    else if (p.body_o == 4) rc = launch_items<T, DH, 4, 4, true>(a, ip, io, st);
     else rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
     return rc || (!p.share && p.So == 1) ? rc : launch_join<T>(a, st);
 }

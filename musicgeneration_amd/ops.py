@@ -1403,7 +1403,7 @@ def paged_append(qkv, kcache, vcache, table, lens, n_heads: int, cos=None, sin=N
         q_ptr = rd = rows = 0
     else:
         _rope_tables_ok(cos, sin, dh, qkv, name)
-        q = torch.empty(*lead, n_heads, dh, dtype=qkv.dtype, device=qkv.device)
+        q = qkv.new_empty((*lead, n_heads, dh))
         q_ptr, rows, rd = q.data_ptr(), cos.shape[0], 2 * cos.shape[1]
     if T:
         check(_on(qkv.device, lambda st: lib.mgx_paged_append(
@@ -1479,7 +1479,7 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
             q = q.clone()
     dt = _dt(q)
     floats = lib.mgx_paged_attn_workspace_floats(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dt)
-    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    ws = q.new_empty(floats, dtype=torch.float32) if floats else None
     check(_on(q.device, lambda s: lib.mgx_paged_attn(
         q.data_ptr(), row, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows), _p(slopes),
         _p(prefix) if prefix_len else None, out.data_ptr(), _p(ws), T, B, R, Hq, Hkv, dh, page, n_pages, width, prefix_len,
@@ -1519,8 +1519,8 @@ def verify_draft(target, tokens, uniforms, draft=None, counts=None):
         _beside(counts, "counts", target, _INT32)
         if counts.shape != (B,):
             raise ValueError(f"{name}: counts {tuple(counts.shape)} must be {(B,)}")
-    out = torch.empty(B, k + 1, dtype=tokens.dtype, device=target.device)
-    accepted = torch.empty(B, dtype=torch.int32, device=target.device)
+    out = tokens.new_empty((B, k + 1))
+    accepted = tokens.new_empty(B, dtype=torch.int32)
     if B:
         ds = draft.stride() if draft is not None else (0, 0)
         check(_on(target.device, lambda st: lib.mgx_verify_draft(
