@@ -1168,13 +1168,14 @@ def adamw_step_multi(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps
 _HALF = {"interleaved": 0, "half": 1}
 
 
-def _on(device, launch):
-    """launch(stream) with `device` current: its current stream is where the tensors' work belongs.  (The raw handle: a
-    torch.cuda.Stream object costs 2 us of the 12 us a small call takes.)"""
-    if device.index == torch.cuda.current_device():
-        return launch(torch._C._cuda_getCurrentRawStream(device.index))
+def _on(device, entry, args):
+    """entry(*args, stream) with `device` current: its current stream is where the tensors' work belongs.  (The raw handle: a
+    torch.cuda.Stream object costs 2 us of the 10 us a small call takes.)"""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
-        return launch(torch._C._cuda_getCurrentRawStream(device.index))
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _beside(t, name, like, dtypes):
@@ -1237,8 +1238,7 @@ def rope_tables(n: int, rotary_dim: int, base: float = 10000.0, scaling=None, fa
         raise RuntimeError("rope_tables: musicgeneration_amd runs on the GPU only; there is no CPU fallback")
     cos = torch.empty(n, half, dtype=torch.float32, device=freq.device)
     sin = torch.empty_like(cos)
-    check(_on(freq.device, lambda st: lib.mgx_rope_tables(_p(freq), _p(cos), _p(sin), n, half, amplitude, st)),
-          "mgx_rope_tables")
+    check(_on(freq.device, lib.mgx_rope_tables, (_p(freq), _p(cos), _p(sin), n, half, amplitude)), "mgx_rope_tables")
     return cos, sin
 
 
@@ -1251,10 +1251,11 @@ def _rotary(x, y, cos, sin, positions, half, transposed):
     if B * S * H == 0:
         return y
     xs, ys = x.stride(), y.stride()
-    check(_on(x.device, lambda st: lib.mgx_rotary(
-        x.data_ptr(), y.data_ptr(), cos.data_ptr(), sin.data_ptr(), _p(positions),
-        0 if positions is None or positions.dtype == torch.int32 else 1, B, S, H, dh, 2 * cos.shape[1], cos.shape[0],
-        xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], half, transposed, _dt(x), st)), "mgx_rotary")
+    P, r = cos.shape
+    pos, pos64 = (None, 0) if positions is None else (positions.data_ptr(), positions.dtype == torch.int64)
+    args = (x.data_ptr(), y.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos, pos64, B, S, H, dh, 2 * r, P, xs[0], xs[1], xs[2],
+            ys[0], ys[1], ys[2], half, transposed, _DT[x.dtype])
+    check(_on(x.device, lib.mgx_rotary, args), "mgx_rotary")
     return y
 
 
@@ -1262,20 +1263,20 @@ class _Rotary(torch.autograd.Function):
     """Linear in x: its gradient is the transposed rotation of the incoming one (and so on, to any order)."""
 
     @staticmethod
-    def forward(ctx, x, cos, sin, positions, half, transposed):
+    def forward(ctx, x, how):
+        cos, sin, positions, half, transposed = how
         ctx.save_for_backward(cos, sin, positions)
-        ctx.cfg = half, transposed
+        ctx.way = half, 1 - transposed
         return _rotary(x, _dense_like(x), cos, sin, positions, half, transposed)
 
     @staticmethod
     def backward(ctx, dy):
-        cos, sin, positions = ctx.saved_tensors
-        half, transposed = ctx.cfg
+        how = (*ctx.saved_tensors, *ctx.way)
         if dy.stride(-1) != 1:
             dy = dy.contiguous()
         if torch.is_grad_enabled():               # create_graph: the gradient is differentiable itself
-            return _Rotary.apply(dy, cos, sin, positions, half, 1 - transposed), None, None, None, None, None
-        return _rotary(dy, _dense_like(dy), cos, sin, positions, half, 1 - transposed), None, None, None, None, None
+            return _Rotary.apply(dy, how), None
+        return _rotary(dy, _dense_like(dy), *how), None
 
 
 def _rotary_args(x, cos, sin, positions, layout, name):
@@ -1309,7 +1310,7 @@ def rotary(x, cos, sin, positions=None, layout: str = "interleaved"):
     positions [B,S] int32 / int64, None: 0..S-1.  Positions outside the tables are clamped to their ends."""
     half = _rotary_args(x, cos, sin, positions, layout, "rotary")
     if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, cos, sin, positions, half, 0)
+        return _Rotary.apply(x, (cos, sin, positions, half, 0))
     return _rotary(x, _dense_like(x), cos, sin, positions, half, 0)
 
 
@@ -1406,10 +1407,10 @@ def paged_append(qkv, kcache, vcache, table, lens, n_heads: int, cos=None, sin=N
         q = qkv.new_empty((*lead, n_heads, dh))
         q_ptr, rows, rd = q.data_ptr(), cos.shape[0], 2 * cos.shape[1]
     if T:
-        check(_on(qkv.device, lambda st: lib.mgx_paged_append(
+        check(_on(qkv.device, lib.mgx_paged_append, (
             qkv.data_ptr(), q_ptr, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows),
             _p(cos), _p(sin), T, B, 0 if cu_rows is not None else lead[1], n_heads, Hkv, dh, rd, page, n_pages, width, rows,
-            offset, _HALF[layout], _dt(qkv), st)), "mgx_paged_append")
+            offset, _HALF[layout], _DT[qkv.dtype])), "mgx_paged_append")
     return q
 
 
@@ -1480,10 +1481,10 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     dt = _dt(q)
     floats = lib.mgx_paged_attn_workspace_floats(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dt)
     ws = q.new_empty(floats, dtype=torch.float32) if floats else None
-    check(_on(q.device, lambda s: lib.mgx_paged_attn(
+    check(_on(q.device, lib.mgx_paged_attn, (
         q.data_ptr(), row, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows), _p(slopes),
         _p(prefix) if prefix_len else None, out.data_ptr(), _p(ws), T, B, R, Hq, Hkv, dh, page, n_pages, width, prefix_len,
-        max_rows, max_len, scale, dt, s)), "mgx_paged_attn")
+        max_rows, max_len, scale, dt)), "mgx_paged_attn")
     return out
 
 
@@ -1523,8 +1524,8 @@ def verify_draft(target, tokens, uniforms, draft=None, counts=None):
     accepted = tokens.new_empty(B, dtype=torch.int32)
     if B:
         ds = draft.stride() if draft is not None else (0, 0)
-        check(_on(target.device, lambda st: lib.mgx_verify_draft(
+        check(_on(target.device, lib.mgx_verify_draft, (
             target.data_ptr(), _p(draft) if k else None, _p(tokens), 1 if tokens.dtype == torch.int64 else 0,
             uniforms.data_ptr(), _p(counts), out.data_ptr(), accepted.data_ptr(), B, k, V, target.stride(0),
-            target.stride(1), ds[0], ds[1], dt, st)), "mgx_verify_draft")
+            target.stride(1), ds[0], ds[1], dt)), "mgx_verify_draft")
     return out, accepted
