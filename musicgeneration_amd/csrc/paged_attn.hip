@@ -956,13 +956,12 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
     }
 }
 
-// BODY: 0 / 1 private with 16 / 32 rows, 2 / 3 shared with 32 / 64 rows a wave, 4 private with 16 rows and as many waves as
-// the LDS of a CU holds tiles for: few items of long sequences, each of which one workgroup takes without a join
+// BODY: 0 / 1 private with 16 / 32 rows, 2 / 3 shared with 32 / 64 rows a wave, 4 private with 16 rows and eight waves (where
+// the LDS holds their tiles): few items of long sequences, each of which one workgroup takes without a join.  (Sixteen waves
+// for heads of 64: 16 sequences of up to 8000 keys 53 instead of 37 us, 128 registers a lane are too few.)
 template <typename T, int DH, int BODY>
 constexpr int waves_of() {
-    if (BODY != 4) return NW;
-    const int fit = 136 * 1024 / (Prod16<T, DH>::KB + Prod16<T, DH>::VB);
-    return fit >= 16 ? 16 : fit >= 8 ? 8 : 4;
+    return BODY == 4 && 8 * (Prod16<T, DH>::KB + Prod16<T, DH>::VB) <= 136 * 1024 ? 8 : NW;
 }
 template <typename T, int DH, int BODY>
 constexpr int body_smem() {
@@ -1179,7 +1178,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
             return parts_of(base, keys, 64, bytes == 4 && DH == 128 ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
                             row_us, join, chunk, us);
         }
-        const int groups = body == 4 ? 512 / (DH * bytes) : 1, slots = body == 4 ? 256 : 512;       // (waves_of) / 4
+        const int groups = body == 4 ? 2 : 1, slots = 512 / groups;       // (waves_of / 4)
         return parts_of(base, keys, 128 * groups, slots, 0.5 * key_bytes * slots / 5.0e6, (bytes == 4 ? 1.8 : 1.0) * key_bytes / (25.0e3 * groups), beside,
                         row_us, join, chunk, us);
     };
