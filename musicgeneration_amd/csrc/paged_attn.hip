@@ -17,6 +17,17 @@
 //            own with the next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
 //   shared   32 rows a wave (32x32 tiles), 128 in all: 64-key tiles in LDS, double buffered, shared by the four waves.
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
+//
+// Measured (library product of 8192^3 bf16: 1172 TFLOP/s; copy: 5.15 TB/s; calls one after another):
+//   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     50 us   (own keys alone 36: 3.8 TB/s, the ragged
+//                                                                           end; prefix alone 32; together they overlap)
+//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s: bound by the issue of vector
+//                                                                           instructions and the clock held under it (1.8 GHz)
+//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        352 us  727 TFLOP/s: the same
+//   16 sequences x 1 row, 8 heads of 64, own <= 2048                        13 us of kernel, 6 of them begin and end
+//   1 sequence, 8 heads of 128, 30001 keys                                  36 us   (3.4 TB/s with the join)
+//   24 x 3 rows fp32, 12 + 4 heads of 64, prefix 1000, own <= 703           16 + 4 us: latency
+// An item costs 5 us of beginning (length, page, keys: three dependent loads) and end; that is what limits splitting.
 #include "attn_mfma_common.h"
 
 namespace {

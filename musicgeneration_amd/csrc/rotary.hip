@@ -9,6 +9,9 @@
 // same unit of HPT heads of one row.  The angles (4 bytes each of cos and sin per pair, twice the bytes of a bf16 value
 // pair) are then loaded once for HPT heads instead of once per head, and HPT vectors are in flight.  Consecutive lanes
 // take consecutive units, then head groups, so a wave's request covers whole heads (128 bytes and more).
+// Measured (a copy of 1 GiB moves 5.15 TB/s): q | k heads of 16 x 2048 rows, 16 heads of 64, bf16: 26 us = 5.1 TB/s;
+// prompts of 16.5 k rows, 32 + 2 x 8 heads of 128, rotated and filed: 78.7 us = 5.15 TB/s; one row for each of 64 sequences:
+// 4.5 us, of which the launch, two dependent loads (length, page) and the row's own are nearly all.
 #include "mgx_common.h"
 
 namespace {
