@@ -6,7 +6,7 @@
 //   Key j of the prefix is row j % page of page prefix[j / page], own key j that of page table[b][j / page]; a page outside
 //   the pool hides its keys.  Softmax statistics and sums are fp32.
 //
-// Keys are numbered through, the prefix's 0..P-1 first.  A work item is (rows, key range): up to 32 or 128 of the rows
+// Keys are numbered through, the prefix's 0..P-1 first.  A work item is (rows, key range): up to 32, 128 or 256 of the rows
 // that read one K/V head - the G = Hq / Hkv query heads of a group are rows of the same tile - against a range of keys.
 //   own items     rows of one sequence, its own keys (all keys, where the prefix is not taken apart)
 //   prefix items  rows of the WHOLE batch, prefix keys: K and V of the prefix are read once per row tile of the batch
@@ -15,19 +15,24 @@
 // operand without leaving the registers (the order of the keys in it is free, V is read in the same one).  Two bodies:
 //   private  <= 16 or 32 rows (16x16 tiles): memory bound.  The waves take alternate 32-key tiles, each through LDS of its
 //            own with the next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
-//   shared   32 rows a wave (32x32 tiles), 128 in all: 64-key tiles in LDS, double buffered, shared by the four waves.
+//            Four waves, or eight where few items have long ranges.
+//   shared   32 or 64 rows a wave (32x32 tiles), 128 or 256 in all: 64-key tiles in LDS, double buffered, shared by the
+//            four waves.
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
 //
 // Measured (library product of 8192^3 bf16: 1172 TFLOP/s; copy: 5.15 TB/s; calls one after another):
 //   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     50 us   (own keys alone 36: 3.8 TB/s, the ragged
 //                                                                           end; prefix alone 32; together they overlap)
-//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s: bound by the issue of vector
-//                                                                           instructions and the clock held under it (1.8 GHz)
-//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        352 us  727 TFLOP/s: the same
-//   16 sequences x 1 row, 8 heads of 64, own <= 2048                        13 us of kernel, 6 of them begin and end
+//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s (147 us without a pause between
+//                                                                           calls): a SIMD issues in 70 % of its busy cycles,
+//                                                                           its matrix unit works in 28 %
+//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        352 us  727 TFLOP/s (385 without a pause): issue
+//                                                                           56 %, matrix unit 31 %, neither full
+//   16 sequences x 1 row, 8 heads of 64, own <= 2048                        14 us of kernel (one key each instead: 6 to 7)
 //   1 sequence, 8 heads of 128, 30001 keys                                  36 us   (3.4 TB/s with the join)
 //   24 x 3 rows fp32, 12 + 4 heads of 64, prefix 1000, own <= 703           16 + 4 us: latency
-// An item costs 5 us of beginning (length, page, keys: three dependent loads) and end; that is what limits splitting.
+// A launch whose items hold one key takes 5.6 us (1 sequence) to 8 us (64, heads of 128): the beginning (length, page, keys:
+// three dependent loads) and the end of an item.  That is what limits splitting; the plan reckons 5 us an item.
 #include "attn_mfma_common.h"
 
 namespace {
