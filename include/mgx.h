@@ -420,7 +420,8 @@ int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const v
  *   token i stays while u_i q_i(x_i) < p_i(x_i); behind the a that stay one token is drawn with u_k from max(p_a - q_a, 0),
  *   or from p_a when all stayed (or nothing is left over): the smallest class whose running sum passes u_k * total
  *   out [B,k+1] (as tokens): the tokens that stay, the drawn one, -1 behind; accepted [B] int32 = a
- *   draft == NULL: drafted tokens were certain (q = one-hot).  Values that are not positive and finite weigh nothing.
+ *   draft == NULL: drafted tokens were certain (q = one-hot).  Values that are not positive and finite weigh nothing;
+ *   a token of such a p does not stay.
  * Products and running sums in fp64, fixed order. */
 int mgx_verify_draft(const void* target, const void* draft, const void* tokens, int tokens_are_int64, const float* uniforms,
                      const int* counts, void* out, int* accepted, int B, int k, long V, long target_stride_b,

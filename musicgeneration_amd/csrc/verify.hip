@@ -3,7 +3,8 @@
 //   test i (in order, i < n): the draft's token x_i stays while u_i q_i(x_i) < p_i(x_i); a = the number that stay
 //   then one token is drawn from  w = max(p_a - q_a, 0)  (a < n)  or  w = p_a  (a = n, or where the former is zero):
 //   the smallest class c with  w_0 + .. + w_c > u_last (w_0 + .. + w_{V-1})
-//   no draft distribution: q is the one-hot of the drafted token.  A value that is not a positive finite number weighs 0.
+//   no draft distribution: q is the one-hot of the drafted token.  A value that is not a positive finite number weighs 0,
+//   and a token of such a p does not stay.
 //
 // Bound by reading one row of p and one of q per sequence: one workgroup per sequence reads them ONCE for the total, and
 // then only walks down: 16 slices -> the slice that holds the target, its 16 sub-slices -> the sub-slice, 64 classes at
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(64 * NW) void verify_draft_kernel(const T* __restri
                 fails = true;                          // a class outside the vocabulary has p = 0
                 if (c >= 0 && c < V) {
                     const double pv = to_f32(tp[i * tsr + c]), qv = dp ? to_f32(dp[i * dsr + c]) : 1.f;
-                    fails = !((double)ub[i] * qv < pv);
+                    fails = !((double)ub[i] * qv < pv && pv > 0.0 && pv < (double)INFINITY);
                 }
             }
             const unsigned long long m = __ballot(fails);

@@ -1496,8 +1496,8 @@ def verify_draft(target, tokens, uniforms, draft=None, counts=None):
     None: they were certain; counts [B] int32: tokens drafted per sequence, None: k.
     Token i stays while u_i q_i(x_i) < p_i(x_i).  Behind the a tokens that stay, one is drawn with uniforms[:, k] from
     max(p_a - q_a, 0), or from p_a when all stayed (or nothing is left over): the smallest class whose running sum (fp64)
-    passes u * total.  Probabilities that are not positive and finite weigh nothing; a drafted class outside [0, V) does
-    not stay.  Returns (out [B,k+1] as tokens: those that stay, the drawn one, -1 behind; accepted [B] int32 = a)."""
+    passes u * total.  Probabilities that are not positive and finite weigh nothing; a drafted class of such a p, or
+    outside [0, V), does not stay.  Returns (out [B,k+1] as tokens: those that stay, the drawn one, -1 behind; accepted [B] int32 = a)."""
     name = "verify_draft"
     if not target.is_cuda:
         raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (target is on {target.device}); there is no CPU fallback")

@@ -137,7 +137,7 @@ def verify(target, tokens, u, draft=None, counts=None):
             if not 0 <= c < V:
                 break
             q = 1.0 if draft is None else float(draft[b, a, c])
-            if not float(u[b, a]) * q < float(target[b, a, c]):
+            if not float(u[b, a]) * q < float(target[b, a, c]) or not float(clean(target[b, a, c])) > 0:
                 break
             out[b, a] = c
             a += 1

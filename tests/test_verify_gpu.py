@@ -93,3 +93,21 @@ def test_verify_draft_replays_in_a_graph():
         torch.cuda.synchronize()
         want, n = verify(p.cpu(), x.cpu(), u.cpu(), q.cpu())
         assert torch.equal(out.cpu(), want) and torch.equal(acc.cpu(), n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_verify_draft_keeps_no_token_without_weight(dtype):
+    """A drafted class whose target probability is not positive and finite does not stay, whatever the draft's is; what is
+    drawn then follows the same rule.  (u_i q_i < p_i alone would keep class 0 of each.)"""
+    from musicgeneration_amd import ops
+    inf = float("inf")
+    p = torch.tensor([[inf, 0.25, 0.75], [0.0, 0.5, 0.5], [-0.25, 1.0, 0.0]], dtype=dtype)[:, None].repeat(1, 2, 1)
+    q = torch.tensor([[0.5, 0.5, 0.0], [-1.0, 0.5, 0.5], [-1.0, 1.0, 0.0]], dtype=dtype)[:, None]
+    x, u = torch.zeros(3, 1, dtype=torch.int64), torch.full((3, 2), 0.5)
+    # left over: (0, 0, .75); nothing, so p: (0, .5, .5), where class 1's running sum does not pass .5; nothing, so p: (0, 1, 0)
+    want = [[2, -1], [2, -1], [1, -1]]
+    for draft in (q, None):
+        got, n = ops.verify_draft(p.cuda(), x.cuda(), u.cuda(), None if draft is None else draft.cuda())
+        assert n.tolist() == [0, 0, 0]
+        # certain drafts: the one-hot takes class 0 away, which weighs nothing: row 0 draws .5 of (.25, .75) -> class 2
+        assert got.tolist() == want
