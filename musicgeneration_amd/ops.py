@@ -1380,7 +1380,7 @@ def paged_append(qkv, kcache, vcache, table, lens, n_heads: int, cos=None, sin=N
     if not qkv.is_cuda:
         raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (qkv is on {qkv.device}); there is no CPU fallback")
     _dt(qkv)
-    _no_grad_of(name, qkv)
+    _no_grad_of(name, qkv, kcache, vcache)
     if not qkv.is_contiguous() or qkv.data_ptr() % 16:
         raise ValueError(f"{name}: qkv must be contiguous and 16-byte aligned")
     n_pages, Hkv, page, dh = _cache_args(kcache, vcache, table, lens, qkv, name)
@@ -1430,7 +1430,7 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     if not q.is_cuda:
         raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (q is on {q.device}); there is no CPU fallback")
     _dt(q)
-    _no_grad_of(name, q, slopes)
+    _no_grad_of(name, q, kcache, vcache, slopes)
     n_pages, Hkv, page, dh = _cache_args(kcache, vcache, table, lens, q, name)
     B, width = table.shape
     if q.dim() != (4 if cu_rows is None else 3) or q.shape[-1] != dh or (cu_rows is None and q.shape[0] != B):

@@ -186,3 +186,15 @@ def test_c_entry_points_refuse():
     for kw in ({"f": n}, {"nn": 0}, {"half": 0}):
         assert tab(**kw) < 0, kw
     assert lib.mgx_last_error_string()
+
+
+def test_caches_and_weights_that_want_a_gradient_are_refused(pointers):
+    """Filing and attention form no gradient: of the caches no more than of q."""
+    qkv, q = E(3, 2, 8 * 64, dtype=BF16), E(3, 2, 4, 64, dtype=BF16)
+    for which in ("kcache", "vcache"):
+        cache = _cache()
+        cache[which].requires_grad_()
+        pointers.append(cache)
+        refuse(RuntimeError, "no gradient", ops.paged_append, qkv, **cache, n_heads=4)
+        refuse(RuntimeError, "no gradient", ops.paged_attn, q, **cache)
+    refuse(RuntimeError, "no gradient", ops.paged_attn, q, **_cache(), slopes=E(4).requires_grad_())
