@@ -27,6 +27,9 @@ int mgx_cu_count();
         }                                       \
     } while (0)
 
+// a launch dimension holds fewer than 2^32 threads
+inline bool grid_fits(long blocks, int threads) { return blocks <= 0xFFFFFFFFL / threads; }
+
 #define MGX_CHECK_LAUNCH(name)                                                        \
     do {                                                                              \
         hipError_t e_ = hipGetLastError();                                            \

@@ -1173,6 +1173,9 @@ inline int parts_of(long base, long keys, long unit, int slots, double key, doub
 }
 
 Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int max_len, int dtype) {
+    max_rows = max_rows < T ? max_rows : (int)T;       // (hints: what is beyond any table or batch says nothing)
+    const int room = P < 1 << 30 ? (1 << 30) - P : 1;
+    max_len = max_len < room ? max_len : room;
     Plan p = {};
     p.rows_only = dh > 128;                            // a wave's sums, q and staged keys no longer fit its registers
     const long G = Hq / Hkv, rows = (long)max_rows * G;
@@ -1228,6 +1231,11 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
         apart_us = (prefix_us > own_us ? prefix_us : own_us) + 4.0;
         if (apart_us < us) p = s;
     }
+    // Row tiles of a sequence beyond what a launch holds go to the same workgroups in turn (many ragged sequences with no
+    // closer bound of their rows than all of them).
+    const long most = 0xFFFFFFFFL / (p.body_o == 4 ? 512 : 256) - CLEARERS - (p.share ? ceil_div((long)Hkv * p.Sp, 8) * 8 * p.rt_p : 0);
+    const long fit = most / ((long)B * Hkv * p.So);
+    if (p.rt_o > fit) p.rt_o = fit > 1 ? (int)fit : 1;
     return p;
 }
 
@@ -1236,7 +1244,7 @@ int launch_items(const PagedArgs& a, long items_p, long items_o, hipStream_t st)
     constexpr int sp = body_smem<T, DH, BODY_P>(), so = body_smem<T, DH, BODY_O>(), smem = sp > so ? sp : so;
     static_assert(smem <= 160 * 1024, "LDS of a CU");
     const long items = items_p + items_o, grid = items + (a.cu ? CLEARERS : 0);
-    MGX_REQUIRE(grid < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
+    MGX_REQUIRE(grid_fits(grid, 64 * waves_of<T, DH, BODY_O>()), MGX_EUNSUPPORTED, "mgx_paged_attn: too many work items");
     if (smem > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_attn_kernel<T, DH, BODY_P, BODY_O, ALIBI>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -1263,7 +1271,7 @@ int launch_join(const PagedArgs& a, hipStream_t st) {
     const int parts = (a.share ? a.Sp : 0) + a.So;
     while ((rows << lq) * L < 65536 && (L << lq) < 256 && 2 * L <= parts) L *= 2;       // a wave on each SIMD
     const long blocks = ceil_div(rows, (256 >> lq) / L);
-    MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
+    MGX_REQUIRE(grid_fits(blocks, 256), MGX_EUNSUPPORTED, "mgx_paged_attn: too many rows");
     hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a, lq, L);
     MGX_CHECK_LAUNCH("paged_join");
     return MGX_OK;
@@ -1328,6 +1336,7 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
     a.rt_p = p.rt_p, a.rt_o = p.rt_o;
     hipStream_t st = (hipStream_t)stream;
     if (p.rows_only) {
+        MGX_REQUIRE(grid_fits(T, 256), MGX_EUNSUPPORTED, "mgx_paged_attn: T=%ld rows of heads wider than 128", T);
         const dim3 grid((unsigned)T, Hq);
         int lpr = 1;
         while (lpr * N < dh) lpr *= 2;

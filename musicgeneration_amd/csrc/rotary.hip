@@ -260,7 +260,7 @@ inline bool wide_units(int dh, int rd, int half, int N) { return dh % N == 0 && 
 template <typename A>
 int launch_units(void (*k)(const A), const A& a, long threads, const char* name, hipStream_t st) {
     const long blocks = (threads + 255) / 256;
-    MGX_REQUIRE(blocks < (1L << 31), MGX_EUNSUPPORTED, "%s: too many rows", name);
+    MGX_REQUIRE(grid_fits(blocks, 256), MGX_EUNSUPPORTED, "%s: too many rows", name);
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, a);
     MGX_CHECK_LAUNCH(name);
     return MGX_OK;
@@ -287,6 +287,7 @@ extern "C" int mgx_rope_tables(const double* freq, float* cos_tab, float* sin_ta
     MGX_REQUIRE(freq && cos_tab && sin_tab, MGX_EINVAL, "mgx_rope_tables: null pointer");
     MGX_REQUIRE(n > 0 && half > 0 && n <= (1L << 38) / half, MGX_EINVAL, "mgx_rope_tables: n=%ld half=%d", n, half);
     const long blocks = (n * half + 255) / 256;
+    MGX_REQUIRE(grid_fits(blocks, 256), MGX_EUNSUPPORTED, "mgx_rope_tables: n=%ld half=%d", n, half);
     hipLaunchKernelGGL(rope_tables_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, freq, cos_tab,
                        sin_tab, n, half, amplitude);
     MGX_CHECK_LAUNCH("rope_tables");

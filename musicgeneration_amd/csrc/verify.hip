@@ -176,6 +176,7 @@ extern "C" int mgx_verify_draft(const void* target, const void* draft, const voi
     MGX_REQUIRE(target && uniforms && out && accepted && (tokens || k == 0), MGX_EINVAL, "mgx_verify_draft: null pointer");
     MGX_REQUIRE(B > 0 && k >= 0 && V > 0 && V < (1L << 31), MGX_EINVAL, "mgx_verify_draft: B=%d k=%d V=%ld", B, k, V);
     MGX_REQUIRE(dtype == MGX_F32 || dtype == MGX_BF16, MGX_EINVAL, "mgx_verify_draft: bad dtype %d", dtype);
+    MGX_REQUIRE(grid_fits(B, 64 * NW), MGX_EUNSUPPORTED, "mgx_verify_draft: B=%d", B);
     hipStream_t st = (hipStream_t)stream;
 #define MGX_VERIFY(T_, I_)                                                                                              \
     hipLaunchKernelGGL((verify_draft_kernel<T_, I_>), dim3(B), dim3(64 * NW), 0, st, (const T_*)target,                 \

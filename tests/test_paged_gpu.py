@@ -370,3 +370,23 @@ def test_serving_run_equals_one_causal_pass(dtype, layout):
         assert torch.equal(tokens.cpu(), want) and torch.equal(taken.cpu(), n)
         lens -= k - taken                      # the rejected rows' slots are filed over in the next step
         history = [torch.cat((history[b], rows[b, :1 + int(n[b])])) for b in range(B)]
+
+
+def test_attn_many_ragged_sequences_without_a_bound_of_their_rows():
+    """More row tiles (8192 sequences x all rows) than a launch holds: keys of zero weigh the same, so a row's output is the
+    mean of its sequence's values, whole numbers: sums of them are exact, the division is off by at most 2 x 2^-24."""
+    from musicgeneration_amd import ops
+    B, T, dh, page = 8192, 300000, 64, 64
+    n = torch.full((B,), T // B, dtype=torch.int64)
+    n[5], n[4000] = 0, T - int(n.sum()) + int(n[4000]) - 100 + int(n[5])         # one empty, one long, 100 rows behind the last
+    cu = torch.cat((torch.zeros(1, dtype=torch.int64), n.cumsum(0))).int().cuda()
+    width = int(-(-n.max() // page))
+    value = torch.arange(B, device="cuda") % 61 + 1
+    kc = torch.zeros(61, 1, page, dh, device="cuda")
+    vc = torch.arange(1, 62, device="cuda").float().view(61, 1, 1, 1).expand(61, 1, page, dh).contiguous()
+    table = (value - 1).int()[:, None].expand(B, width).contiguous()
+    out = ops.paged_attn(torch.randn(T, 1, dh, device="cuda"), kc, vc, table, n.int().cuda(), cu_rows=cu)
+    last = int(cu[-1])
+    want = value.repeat_interleave(n.cuda(), output_size=last).double()[:, None, None]
+    assert last == T - 100 and not out[last:].any()
+    assert float(((out[:last].double() - want).abs() / want).max()) <= 2 * 2.0 ** -24

@@ -198,3 +198,18 @@ def test_caches_and_weights_that_want_a_gradient_are_refused(pointers):
         refuse(RuntimeError, "no gradient", ops.paged_append, qkv, **cache, n_heads=4)
         refuse(RuntimeError, "no gradient", ops.paged_attn, q, **cache)
     refuse(RuntimeError, "no gradient", ops.paged_attn, q, **_cache(), slopes=E(4).requires_grad_())
+
+
+def test_launches_beyond_the_grid_are_refused():
+    """2^32 threads a launch dimension: more is refused as unsupported, before a launch is tried (the pointers are not memory)."""
+    a, b, n, unsupported = 16, 32, None, -2
+    big = 1 << 24
+    assert lib.mgx_rotary(a, a, a, a, n, 0, 1, 2 ** 31 - 1, 1, 64, 64, 2 ** 31 - 1, 64, 64, 64, 64, 64, 64, 0, 0, 1, n) == unsupported
+    assert lib.mgx_rope_tables(a, a, a, 1 << 31, 2, 1.0, n) == unsupported
+    assert lib.mgx_verify_draft(a, n, a, 0, a, n, a, a, 1 << 22, 1, 4, 8, 4, 0, 0, 0, n) == unsupported
+    append = lambda T, dh, rd: lib.mgx_paged_append(a, a, a, b, a, a, n, a, a, T, T, 1, 8, 8, dh, rd, 4, 2, 2, 4, 0, 0, 1, n)   # noqa: E731
+    assert append(1 << 28, 128, 128) == unsupported
+    attn = lambda T, Hq, dh, cu=n, R=1, B=None, mr=1: lib.mgx_paged_attn(   # noqa: E731
+        a, Hq * dh, a, b, a, a, cu, n, n, a, a, T, T if B is None else B, R, Hq, 1, dh, 4, 2, 2, 0, mr, 8, 1.0, 1, n)
+    assert attn(big, 1, 136) == unsupported             # a workgroup a row
+    assert attn(big, 1, 64) == unsupported              # a workgroup a sequence
