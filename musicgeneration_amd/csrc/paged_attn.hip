@@ -1111,7 +1111,7 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, 
         if (see) {
             s = s * a.scale + slope * (float)(j - i);
             const float mn = fmaxf(m, s);
-            const float alpha = mn == -INFINITY ? 1.f : expf(m - mn), p = mn == -INFINITY ? 0.f : expf(s - mn);
+            const float alpha = mn == -INFINITY ? 1.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);      // (NaN stays)
             l = l * alpha + p;
             m = mn;
 #pragma unroll

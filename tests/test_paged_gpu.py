@@ -390,3 +390,20 @@ def test_attn_many_ragged_sequences_without_a_bound_of_their_rows():
     want = value.repeat_interleave(n.cuda(), output_size=last).double()[:, None, None]
     assert last == T - 100 and not out[last:].any()
     assert float(((out[:last].double() - want).abs() / want).max()) <= 2 * 2.0 ** -24
+
+
+def test_attn_a_row_that_is_not_a_number_stays_alone():
+    """A padded batch: q of one sequence is NaN.  The prefix's tiles hold rows of all sequences; the others' outputs are the same."""
+    from musicgeneration_amd import ops
+    for dtype, B, R, Hq, Hkv, dh, P in ((BF16, 48, 1, 8, 2, 64, 700), (F32, 12, 3, 4, 2, 64, 300), (BF16, 70, 6, 4, 2, 64, 515), (BF16, 40, 4, 8, 2, 128, 600),
+                                        (BF16, 3, 2, 4, 2, 136, 40)):
+        k, v, table, prefix, g = _pool([70] * B, Hkv, 16, dh, dtype, P, seed=B)
+        q = torch.randn(B, R, Hq, dh, generator=g).to(dtype).cuda()
+        lens = torch.full((B,), 70, dtype=torch.int32).cuda()
+        call = lambda x: ops.paged_attn(x, k.cuda(), v.cuda(), table.cuda(), lens, prefix=prefix.cuda(), prefix_len=P)   # noqa: E731
+        clean = call(q)
+        q[1], q[B - 1, 0] = NAN, math.inf
+        got = call(q)
+        stay = [b for b in range(B) if b not in (1, B - 1)]
+        assert torch.equal(got[stay], clean[stay]), (dtype, B, R, dh)
+        assert not torch.isfinite(got[1].float()).any()
