@@ -407,3 +407,44 @@ def test_attn_a_row_that_is_not_a_number_stays_alone():
         stay = [b for b in range(B) if b not in (1, B - 1)]
         assert torch.equal(got[stay], clean[stay]), (dtype, B, R, dh)
         assert not torch.isfinite(got[1].float()).any()
+
+
+def test_serving_on_two_streams_from_two_threads():
+    """Calls of two threads, each on a stream of its own behind work that fills its inputs late, equal the same calls alone."""
+    import threading
+    from musicgeneration_amd import ops
+    B, R, Hq, Hkv, dh, P = 6, 2, 8, 2, 64, 200
+    cos, sin = ops.rope_tables(P + 400, dh)
+
+    def run(seed, out):
+        k, v, table, prefix, g = _pool([330] * B, Hkv, 16, dh, BF16, P, seed=seed)
+        src = torch.randn(B, R, (Hq + 2 * Hkv) * dh, generator=g).bfloat16().cuda()
+        k, v, table, prefix = k.cuda(), v.cuda(), table.cuda(), prefix.cuda()
+        lens = torch.full((B,), 330, dtype=torch.int32, device="cuda")
+        big = torch.ones(1 << 24, device="cuda")
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream), torch.no_grad():
+            for _ in range(8):
+                for _ in range(6):
+                    big = big * 1.0
+                qkv = src * big[:1].bfloat16()
+                q = ops.paged_append(qkv, k, v, table, lens, Hq, cos, sin, offset=P)
+                res = ops.paged_attn(q, k, v, table, lens, prefix=prefix, prefix_len=P)
+                prob = res.float().reshape(B, R, -1).softmax(-1)
+                tok, acc = ops.verify_draft(prob, torch.zeros(B, R - 1, dtype=torch.int64, device="cuda"), torch.full((B, R), 0.5, device="cuda"))
+                out.append((res, ops.rotary(res, cos, sin), tok, acc))
+            stream.synchronize()
+
+    alone, both = [[], []], [[], []]
+    for i in range(2):
+        run(i, alone[i])
+    threads = [threading.Thread(target=run, args=(i, both[i])) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for a, b in zip(alone, both):
+        assert len(a) == len(b) == 8
+        for x, y in zip(a, b):
+            assert all(torch.equal(s, t) for s, t in zip(x, y))
