@@ -23,10 +23,10 @@
 // Measured (library product of 8192^3 bf16: 1172 TFLOP/s; copy: 5.15 TB/s; calls one after another):
 //   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     50 us   (own keys alone 36: 3.8 TB/s, the ragged
 //                                                                           end; prefix alone 32; together they overlap)
-//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s (147 us without a pause between
+//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s (143 us without a pause between
 //                                                                           calls): a SIMD issues in 70 % of its busy cycles,
 //                                                                           its matrix unit works in 28 %
-//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        352 us  727 TFLOP/s (385 without a pause): issue
+//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        352 us  727 TFLOP/s (381 without a pause): issue
 //                                                                           56 %, matrix unit 31 %, neither full
 //   16 sequences x 1 row, 8 heads of 64, own <= 2048                        14 us of kernel (one key each instead: 6 to 7)
 //   1 sequence, 8 heads of 128, 30001 keys                                  36 us   (3.4 TB/s with the join)
