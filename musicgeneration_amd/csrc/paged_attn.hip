@@ -15,7 +15,7 @@
 // operand without leaving the registers (the order of the keys in it is free, V is read in the same one).  Two bodies:
 //   private  <= 16 or 32 rows (16x16 tiles): memory bound.  The waves take alternate 32-key tiles, each through LDS of its
 //            own with the next tile's loads in flight in registers: no barrier in the loop; waves are joined once at the end.
-//            Four waves, or eight where few items have long ranges.
+//            Four waves, or eight where few items have long ranges; two for fp32 heads wider than 128 (LDS).
 //   shared   32 or 64 rows a wave (32x32 tiles), 128 or 256 in all: 64-key tiles in LDS, double buffered, shared by the
 //            four waves.
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
@@ -30,6 +30,8 @@
 //                                                                           56 %, matrix unit 31 %, neither full
 //   16 sequences x 1 row, 8 heads of 64, own <= 2048                        14 us of kernel (one key each instead: 6 to 7)
 //   1 sequence, 8 heads of 128, 30001 keys                                  36 us   (3.4 TB/s with the join)
+//   16 sequences x 1 row, 8 heads of 256, own <= 2048                       36 us   (3.7 TB/s)
+//   3 prompts of 1..500 rows, 8 + 2 heads of 256, behind 500 keys           64 us   (26 with heads of 128)
 //   24 x 3 rows fp32, 12 + 4 heads of 64, prefix 1000, own <= 703           16 + 4 us: latency
 // A launch whose items hold one key takes 5.6 us (1 sequence) to 8 us (64, heads of 128): the beginning (length, page, keys:
 // three dependent loads) and the end of an item.  That is what limits splitting; the plan reckons 5 us an item.
@@ -977,6 +979,7 @@ __device__ __forceinline__ void shared_item(const PagedArgs& a, const Item& it, 
 // for heads of 64: 16 sequences of up to 8000 keys 53 instead of 37 us, 128 registers a lane are too few.)
 template <typename T, int DH, int BODY>
 constexpr int waves_of() {
+    if (DH == 256 && sizeof(T) == 4) return 2;
     return BODY == 4 && 8 * (Prod16<T, DH>::KB + Prod16<T, DH>::VB) <= 136 * 1024 ? 8 : NW;
 }
 template <typename T, int DH, int BODY>
@@ -1074,79 +1077,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a, int 
     put4((T*)a.out + row * a.dh + d0, x);
 }
 
-// Heads wider than 128: one workgroup of 4 waves per (row, head); a key row is spread over lpr lanes, 16 bytes each.
-template <typename T>
-__global__ __launch_bounds__(256) void paged_attn_row_kernel(const PagedArgs a, int lpr) {
-    constexpr int N = 16 / sizeof(T);
-    __shared__ float part[4][256 + 2];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const long t = blockIdx.x;
-    const int h = blockIdx.y, hk = h / (a.Hq / a.Hkv);
-    int b, r, n;
-    const bool real = find_row(a, t, b, r, n);
-    const int own = real ? min(max(sane(a.lens[b]) - n + r + 1, 0), a.width * a.page) : 0;
-    const int keys = real ? a.P + own : 0, i = keys - 1;
-    const int sub = lane / lpr, ch = lane % lpr, rpl = 64 / lpr;
-    const bool has = ch * N < a.dh;
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
-    float q[N], acc[N], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        q[k] = has && real ? to_f32(((const T*)a.q)[t * a.qs + (long)h * a.dh + ch * N + k]) : 0.f;
-        acc[k] = 0.f;
-    }
-    for (int j0 = w * rpl; j0 < keys; j0 += 4 * rpl) {
-        const int j = j0 + sub, jo = j - a.P;
-        int pg = -1;
-        if (j < keys) pg = jo < 0 ? a.prefix[j / a.page] : a.table[(long)b * a.width + jo / a.page];
-        const bool see = (unsigned)pg < (unsigned)a.n_pages;
-        const long at = (((long)pg * a.Hkv + hk) * a.page + (jo < 0 ? j : jo) % a.page) * a.dh + ch * N;
-        float s = 0.f, v[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            v[k] = see && has ? to_f32(((const T*)a.vc)[at + k]) : 0.f;
-            s = fmaf(q[k], see && has ? to_f32(((const T*)a.kc)[at + k]) : 0.f, s);
-        }
-        for (int o = 1; o < lpr; o <<= 1) s += __shfl_xor(s, o, 64);
-        if (see) {
-            s = s * a.scale + slope * (float)(j - i);
-            const float mn = fmaxf(m, s);
-            const float alpha = mn == -INFINITY ? 1.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);      // (NaN stays)
-            l = l * alpha + p;
-            m = mn;
-#pragma unroll
-            for (int k = 0; k < N; ++k) acc[k] = fmaf(p, v[k], acc[k] * alpha);
-        }
-    }
-    for (int o = lpr; o < 64; o <<= 1) {
-        const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(m, m2);
-        const float a1 = mn == -INFINITY ? 1.f : expf(m - mn), a2 = mn == -INFINITY ? 1.f : expf(m2 - mn);
-        l = l * a1 + l2 * a2;
-#pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] = acc[k] * a1 + __shfl_xor(acc[k], o, 64) * a2;
-        m = mn;
-    }
-    if (sub == 0 && has) {
-#pragma unroll
-        for (int k = 0; k < N; ++k) part[w][ch * N + k] = acc[k];
-        if (ch == 0) part[w][256] = m, part[w][257] = l;
-    }
-    __syncthreads();
-    if (tid < a.dh) {
-        const float mm = fmaxf(fmaxf(part[0][256], part[1][256]), fmaxf(part[2][256], part[3][256]));
-        float num = 0.f, den = 0.f;
-        for (int ww = 0; ww < 4; ++ww) {
-            const float f = part[ww][256] == mm ? 1.f : expf(part[ww][256] - mm);
-            num = fmaf(part[ww][tid], f, num);
-            den = fmaf(part[ww][257], f, den);
-        }
-        ((T*)a.out)[(t * a.Hq + h) * a.dh + tid] = from_f32<T>(den == 0.f ? 0.f : num / den);
-    }
-}
-
 // ---- the split: how rows and keys become work items -------------------------------------------------------------------
 struct Plan {
-    bool rows_only;                  // the row kernel
     int share, Sp, So, chunk_p, chunk_o, rt_p, rt_o, body_p, body_o;
 };
 
@@ -1177,12 +1109,12 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     const int room = P < 1 << 30 ? (1 << 30) - P : 1;
     max_len = max_len < room ? max_len : room;
     Plan p = {};
-    p.rows_only = dh > 128;                            // a wave's sums, q and staged keys no longer fit its registers
     const long G = Hq / Hkv, rows = (long)max_rows * G;
-    const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : 128;
+    const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : dh <= 128 ? 128 : 256;
     // 64 rows a wave share the reads, the page look-ups and the staging of a tile (bf16 heads of 64: prefix items of 3840 rows
     // and 16385 keys: 129 -> 112 us); with 128 sums a row more they would not fit two waves a SIMD
-    auto body_of = [&](long r) { return r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
+    // (heads of 256 fill a wave's registers and half of the LDS: private bodies alone, fp32 16 rows at most)
+    auto body_of = [&](long r) { return DH == 256 ? (r <= 16 || bytes == 4 ? 0 : 1) : r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
     auto tile_rows = [](int body) { return body == 4 ? 16L : body >= 2 ? 32L * NW * (body - 1) : 16L * (body + 1); };
     const double row_us = T * Hq * (dh + 2.0) * 8.0 / 4.2e6;
     const double key_bytes = 2.0 * dh * bytes;
@@ -1197,7 +1129,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
             return parts_of(base, keys, 64, bytes == 4 && DH == 128 ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
                             row_us, join, chunk, us);
         }
-        const int groups = body == 4 ? 2 : 1, slots = 512 / groups;       // (waves_of / 4)
+        const int groups = body == 4 ? 2 : 1, slots = (DH == 256 ? 256 : 512) / groups;       // (waves_of / 4)
         return parts_of(base, keys, 128 * groups, slots, 0.5 * key_bytes * slots / 5.0e6, (bytes == 4 ? 1.8 : 1.0) * key_bytes / (25.0e3 * groups), beside,
                         row_us, join, chunk, us);
     };
@@ -1281,15 +1213,16 @@ template <typename T, int DH>
 int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
     const long ip = p.share ? ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p : 0, io = (long)a.B * a.Hkv * p.rt_o * p.So;
     int rc;
-    if constexpr (sizeof(T) == 2 && DH == 64) {
-        if (p.body_p == 3) {
-            rc = a.slopes ? launch_wide<T, DH, 3, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, 3, false>(a, p.body_o, ip, io, st);
-            return rc || (!p.share && p.So == 1) ? rc : launch_join<T>(a, st);
-        }
+    if constexpr (DH == 256) {
+        if constexpr (sizeof(T) == 2) rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
+        else rc = launch_items<T, DH, 0, 0, true>(a, ip, io, st);
+    } else {
+        constexpr int TALL = sizeof(T) == 2 && DH == 64 ? 3 : 2;          // (body 3: bf16 heads of 64 alone)
+        if (p.body_p == 3) rc = a.slopes ? launch_wide<T, DH, TALL, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, TALL, false>(a, p.body_o, ip, io, st);
+        else if (p.body_p == 2) rc = a.slopes ? launch_wide<T, DH, 2, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, 2, false>(a, p.body_o, ip, io, st);
+        else if (p.body_o == 4) rc = launch_items<T, DH, 4, 4, true>(a, ip, io, st);
+        else rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
     }
-    if (p.body_p == 2) rc = a.slopes ? launch_wide<T, DH, 2, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, 2, false>(a, p.body_o, ip, io, st);
-    else if (p.body_o == 4) rc = launch_items<T, DH, 4, 4, true>(a, ip, io, st);
-    else rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
     return rc || (!p.share && p.So == 1) ? rc : launch_join<T>(a, st);
 }
 
@@ -1299,7 +1232,7 @@ extern "C" long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, 
                                                 int max_len, int dtype) {
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || dh <= 0 || max_rows <= 0 || max_len <= 0 || prefix_len < 0) return 0;
     const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
-    if (p.rows_only || (!p.share && p.So == 1)) return 0;
+    if (!p.share && p.So == 1) return 0;
     return (p.So + p.Sp) * T * Hq * (dh + 2L);
 }
 
@@ -1324,7 +1257,7 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
                 "mgx_paged_attn: tensors must be 16-byte aligned");
     MGX_REQUIRE(Hq <= 65535 && T * Hq < (1L << 30), MGX_EUNSUPPORTED, "mgx_paged_attn: T=%ld rows of Hq=%d heads", T, Hq);
     const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
-    MGX_REQUIRE(workspace || p.rows_only || (!p.share && p.So == 1), MGX_EINVAL, "mgx_paged_attn: no workspace");
+    MGX_REQUIRE(workspace || (!p.share && p.So == 1), MGX_EINVAL, "mgx_paged_attn: no workspace");
     MGX_REQUIRE((long)n_pages * Hkv * page < 0xFFFFFFFFL, MGX_EUNSUPPORTED, "mgx_paged_attn: pool of more than 2^32 rows");
     PagedArgs a = {};
     a.q = q, a.kc = kcache, a.vc = vcache, a.out = out;
@@ -1335,18 +1268,8 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
     a.share = p.share, a.Sp = p.Sp, a.So = p.So, a.chunk_p = p.chunk_p, a.chunk_o = p.chunk_o;
     a.rt_p = p.rt_p, a.rt_o = p.rt_o;
     hipStream_t st = (hipStream_t)stream;
-    if (p.rows_only) {
-        MGX_REQUIRE(grid_fits(T, 256), MGX_EUNSUPPORTED, "mgx_paged_attn: T=%ld rows of heads wider than 128", T);
-        const dim3 grid((unsigned)T, Hq);
-        int lpr = 1;
-        while (lpr * N < dh) lpr *= 2;
-        if (dtype == MGX_F32) hipLaunchKernelGGL((paged_attn_row_kernel<float>), grid, dim3(256), 0, st, a, lpr);
-        else hipLaunchKernelGGL((paged_attn_row_kernel<bf16_t>), grid, dim3(256), 0, st, a, lpr);
-        MGX_CHECK_LAUNCH("paged_attn_row");
-        return MGX_OK;
-    }
     a.acc = workspace;
     a.ml = workspace + (p.So + p.Sp) * T * Hq * (long)dh;
-    if (dtype == MGX_F32) return dh <= 64 ? launch_paged<float, 64>(a, p, st) : launch_paged<float, 128>(a, p, st);
-    return dh <= 64 ? launch_paged<bf16_t, 64>(a, p, st) : launch_paged<bf16_t, 128>(a, p, st);
+    if (dtype == MGX_F32) return dh <= 64 ? launch_paged<float, 64>(a, p, st) : dh <= 128 ? launch_paged<float, 128>(a, p, st) : launch_paged<float, 256>(a, p, st);
+    return dh <= 64 ? launch_paged<bf16_t, 64>(a, p, st) : dh <= 128 ? launch_paged<bf16_t, 128>(a, p, st) : launch_paged<bf16_t, 256>(a, p, st);
 }
