@@ -31,7 +31,7 @@
 //   16 sequences x 1 row, 8 heads of 64, own <= 2048                        14 us of kernel (one key each instead: 6 to 7)
 //   1 sequence, 8 heads of 128, 30001 keys                                  36 us   (3.4 TB/s with the join)
 //   16 sequences x 1 row, 8 heads of 256, own <= 2048                       36 us   (3.7 TB/s)
-//   3 prompts of 1..500 rows, 8 + 2 heads of 256, behind 500 keys           64 us   (26 with heads of 128)
+//   9 prompts of 1..1500 rows, 16 + 2 heads of 256, behind 4001 keys        1.06 ms 480 TFLOP/s
 //   24 x 3 rows fp32, 12 + 4 heads of 64, prefix 1000, own <= 703           16 + 4 us: latency
 // A launch whose items hold one key takes 5.6 us (1 sequence) to 8 us (64, heads of 128): the beginning (length, page, keys:
 // three dependent loads) and the end of an item.  That is what limits splitting; the plan reckons 5 us an item.
@@ -1113,8 +1113,10 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     const int bytes = dtype == MGX_F32 ? 4 : 2, DH = dh <= 64 ? 64 : dh <= 128 ? 128 : 256;
     // 64 rows a wave share the reads, the page look-ups and the staging of a tile (bf16 heads of 64: prefix items of 3840 rows
     // and 16385 keys: 129 -> 112 us); with 128 sums a row more they would not fit two waves a SIMD
-    // (heads of 256 fill a wave's registers and half of the LDS: private bodies alone, fp32 16 rows at most)
-    auto body_of = [&](long r) { return DH == 256 ? (r <= 16 || bytes == 4 ? 0 : 1) : r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
+    // Heads of 256, one workgroup a CU: 32 private rows a wave spill (16 sequences x 32 rows: 47 instead of 32 us); shared tiles
+    // from 192 rows of a sequence on (16 sequences behind 2000 keys: 64 rows 47 instead of 36 us, 128 52 / 51, 256 84 / 88, long
+    // prompts 1.06 / 2.46 ms), not in fp32 (LDS), and not for a prefix, beside own items (256 rows x 8192 keys 165 / 152 us)
+    auto body_of = [&](long r) { return DH == 256 ? (r < 192 || bytes == 4 ? 0 : 2) : r <= 16 ? 0 : r <= 32 ? 1 : bytes == 2 && DH == 64 && r >= 192 ? 3 : 2; };
     auto tile_rows = [](int body) { return body == 4 ? 16L : body >= 2 ? 32L * NW * (body - 1) : 16L * (body + 1); };
     const double row_us = T * Hq * (dh + 2.0) * 8.0 / 4.2e6;
     const double key_bytes = 2.0 * dh * bytes;
@@ -1126,7 +1128,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
     auto parts = [&](long base, long keys, int body, bool join, double beside, int& chunk, double& us) {
         if (body == 2 || body == 3) {
             const double key = bytes == 4 ? (DH == 64 ? 0.11 : 0.22) : body == 3 ? 0.047 : DH == 64 ? 0.028 : 0.04;
-            return parts_of(base, keys, 64, bytes == 4 && DH == 128 ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
+            return parts_of(base, keys, 64, DH == 256 || (bytes == 4 && DH == 128) ? 256 : 512, key, (beside > 0.0 ? 0.8 : 0.6) * key, beside,
                             row_us, join, chunk, us);
         }
         const int groups = body == 4 ? 2 : 1, slots = (DH == 256 ? 256 : 512) / groups;       // (waves_of / 4)
@@ -1153,7 +1155,7 @@ Plan plan_of(long T, int B, int Hq, int Hkv, int dh, int P, int max_rows, int ma
         Plan s = p;
         double own_us, prefix_us;
         s.share = 1;
-        s.body_p = body_of(T * G);
+        s.body_p = DH == 256 ? 0 : body_of(T * G);
         int body = body_of(rows);
         if (s.body_p == 1 || body > s.body_p) body = s.body_p;           // (fewer instances: a body of more rows takes less)
         if (s.body_p == 3 && body == 2) body = 3;
@@ -1214,8 +1216,10 @@ int launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
     const long ip = p.share ? ceil_div((long)a.Hkv * p.Sp, 8) * 8 * p.rt_p : 0, io = (long)a.B * a.Hkv * p.rt_o * p.So;
     int rc;
     if constexpr (DH == 256) {
-        if constexpr (sizeof(T) == 2) rc = p.body_p == 1 ? launch_items<T, DH, 1, 1, true>(a, ip, io, st) : launch_items<T, DH, 0, 0, true>(a, ip, io, st);
-        else rc = launch_items<T, DH, 0, 0, true>(a, ip, io, st);
+        if constexpr (sizeof(T) == 2) {
+            if (p.body_p == 2) rc = a.slopes ? launch_items<T, DH, 2, 2, true>(a, ip, io, st) : launch_items<T, DH, 2, 2, false>(a, ip, io, st);
+            else rc = launch_items<T, DH, 0, 0, true>(a, ip, io, st);
+        } else rc = launch_items<T, DH, 0, 0, true>(a, ip, io, st);
     } else {
         constexpr int TALL = sizeof(T) == 2 && DH == 64 ? 3 : 2;          // (body 3: bf16 heads of 64 alone)
         if (p.body_p == 3) rc = a.slopes ? launch_wide<T, DH, TALL, true>(a, p.body_o, ip, io, st) : launch_wide<T, DH, TALL, false>(a, p.body_o, ip, io, st);

@@ -448,3 +448,37 @@ def test_serving_on_two_streams_from_two_threads():
         assert len(a) == len(b) == 8
         for x, y in zip(a, b):
             assert all(torch.equal(s, t) for s, t in zip(x, y))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Hq,Hkv,dh", [(4, 1, 256), (6, 2, 136), (3, 3, 192)])
+@pytest.mark.parametrize("P", [0, 77])
+def test_attn_wide_heads_of_many_rows(dtype, Hq, Hkv, dh, P):
+    """Heads wider than 128: prompts whose rows fill tiles of every size (alone, and many short ones behind a prefix)."""
+    cu, lens = [0, 1, 1, 70, 81], [1, 5, 69, 140]
+    k, v, table, prefix, g = _pool(lens, Hkv, 16, dh, dtype, P, seed=dh + P)
+    q = torch.randn(85, Hq, dh, generator=g).to(dtype)
+    slopes = torch.rand(Hq, generator=g)
+    for s in (None, slopes):
+        out = _attend_both(q, k, v, table, lens, s, cu, prefix=prefix, P=P)
+        assert not out[81:].any()
+        _attend_both(q, k, v, table, lens, s, cu, prefix=prefix, P=P, max_rows=1, max_len=1)
+    lens = [20] * 24
+    k, v, table, prefix, g = _pool(lens, Hkv, 16, dh, dtype, P, seed=dh)
+    _attend_both(torch.randn(24, 3, Hq, dh, generator=g).to(dtype), k, v, table, lens, slopes, prefix=prefix, P=P)
+
+
+def test_attn_wide_heads_what_a_row_does_not_see_has_no_effect():
+    """As above for narrower heads, with enough rows for the shared tiles."""
+    from musicgeneration_amd import ops
+    R, n, dh = 48, 90, 256
+    k, v, table, _, g = _pool([n], 1, 16, dh, BF16, seed=2)
+    q = torch.randn(1, R, 2, dh, generator=g).bfloat16().cuda()
+    lens = torch.tensor([n], dtype=torch.int32).cuda()
+    clean = ops.paged_attn(q, k.cuda(), v.cuda(), table.cuda(), lens)
+    for row in (1, 20, 47):
+        j = n - R + row
+        k2, v2 = k.clone(), v.clone()
+        v2[table[0, j // 16], :, j % 16, 200] = math.inf
+        got = ops.paged_attn(q, k2.cuda(), v2.cuda(), table.cuda(), lens)
+        assert torch.equal(got[:, :row], clean[:, :row]) and not torch.isfinite(got[:, row:, :, 200].float()).any()
