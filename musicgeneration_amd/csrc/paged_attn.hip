@@ -21,8 +21,8 @@
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
 //
 // Measured (library product of 8192^3 bf16: 1172 TFLOP/s; copy: 5.15 TB/s; calls one after another):
-//   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     50 us   (own keys alone 36: 3.8 TB/s, the ragged
-//                                                                           end; prefix alone 32; together they overlap)
+//   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     50 us   (own keys alone 36: 3.8 TB/s; prefix alone
+//                                                                           32; together they overlap in part)
 //   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s (143 us without a pause between
 //                                                                           calls): a SIMD issues in 70 % of its busy cycles,
 //                                                                           its matrix unit works in 28 %
