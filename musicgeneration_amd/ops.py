@@ -12,6 +12,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, check
@@ -1191,12 +1192,17 @@ def _beside(t, name, like, dtypes):
 _FP32, _INT32, _INTS = (torch.float32,), (torch.int32,), (torch.int32, torch.int64)
 
 
+def _has_tangent(*ts):
+    """Whether forward-mode differentiation is on and one of ts carries a tangent (such a tensor need not require grad)."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def _rope_tables_ok(cos, sin, dh, like, name):
     _beside(cos, "cos", like, _FP32)
     _beside(sin, "sin", like, _FP32)
     if cos.dim() != 2 or cos.shape != sin.shape or not 0 < 2 * cos.shape[1] <= dh or cos.shape[0] == 0:
         raise ValueError(f"{name}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [positions, rd/2], rd <= {dh}")
-    if cos.requires_grad or sin.requires_grad:
+    if cos.requires_grad or sin.requires_grad or _has_tangent(cos, sin):
         raise ValueError(f"{name}: no gradient is formed for cos and sin")
 
 
@@ -1260,23 +1266,34 @@ def _rotary(x, y, cos, sin, positions, half, transposed):
 
 
 class _Rotary(torch.autograd.Function):
-    """Linear in x: its gradient is the transposed rotation of the incoming one (and so on, to any order)."""
+    """Linear in x: its gradient is the transposed rotation of the incoming one (and so on, to any order), its tangent the
+    rotation of x's."""
 
     @staticmethod
     def forward(ctx, x, how):
         cos, sin, positions, half, transposed = how
         ctx.save_for_backward(cos, sin, positions)
+        ctx.how = how
         ctx.way = half, 1 - transposed
         return _rotary(x, _dense_like(x), cos, sin, positions, half, transposed)
 
     @staticmethod
+    def jvp(ctx, dx, _):
+        return _turned(dx, ctx.how)
+
+    @staticmethod
     def backward(ctx, dy):
-        how = (*ctx.saved_tensors, *ctx.way)
-        if dy.stride(-1) != 1:
-            dy = dy.contiguous()
-        if torch.is_grad_enabled():               # create_graph: the gradient is differentiable itself
-            return _Rotary.apply(dy, how), None
-        return _rotary(dy, _dense_like(dy), *how), None
+        return _turned(dy, (*ctx.saved_tensors, *ctx.way)), None
+
+
+def _turned(x, how):
+    """The rotation of x (any strides): differentiable where x is on a graph or carries a tangent, as the gradient of a
+    gradient's graph and a tangent with a graph of its own are."""
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
+        return _Rotary.apply(x, how)
+    return _rotary(x, _dense_like(x), *how)
 
 
 def _rotary_args(x, cos, sin, positions, layout, name):
@@ -1303,15 +1320,13 @@ def _rotary_args(x, cos, sin, positions, layout, name):
 
 def rotary(x, cos, sin, positions=None, layout: str = "interleaved"):
     """Rotary positions of x [B,S,H,dh] (any strides, unit stride in dh: the q | k heads of a packed projection are one
-    view): a new dense tensor; differentiable in x.
+    view): a new dense tensor; differentiable in x, in reverse and forward mode.
 
     cos, sin [P, rd/2] fp32 (rope_tables); the first rd <= dh values of a head are turned, the rest copied.
     layout: "interleaved" pairs (2i, 2i+1), "half" pairs (i, i + rd/2).
     positions [B,S] int32 / int64, None: 0..S-1.  Positions outside the tables are clamped to their ends."""
     half = _rotary_args(x, cos, sin, positions, layout, "rotary")
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, (cos, sin, positions, half, 0))
-    return _rotary(x, _dense_like(x), cos, sin, positions, half, 0)
+    return _turned(x, (cos, sin, positions, half, 0))
 
 
 def _overlaps(x) -> bool:
@@ -1329,6 +1344,8 @@ def rotary_(x, cos, sin, positions=None, layout: str = "interleaved", transposed
     half = _rotary_args(x, cos, sin, positions, layout, "rotary_")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("rotary_ is not seen by autograd: use rotary, or torch.no_grad()")
+    if _has_tangent(x):
+        raise RuntimeError("rotary_ turns no tangent: use rotary")
     if _overlaps(x):
         raise ValueError("rotary_: elements of x share memory")
     return _rotary(x, x, cos, sin, positions, half, 1 if transposed else 0)
@@ -1340,6 +1357,8 @@ def rotary_(x, cos, sin, positions=None, layout: str = "interleaved", transposed
 def _no_grad_of(name, *ts):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise RuntimeError(f"{name} forms no gradient: call it under torch.no_grad()")
+    if _has_tangent(*ts):
+        raise RuntimeError(f"{name} forms no derivative: an input carries a tangent")
 
 
 def _cache_args(kcache, vcache, table, lens, like, name):

@@ -232,6 +232,8 @@ gemm_nt.register_autograd(_gemm_backward, setup_context=_gemm_setup)
 def rotary(x: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None, layout: str = "interleaved",
            transposed: bool = False) -> Tensor:
     half = ops._rotary_args(x, cos, sin, positions, layout, "rotary")
+    if ops._has_tangent(x):
+        raise RuntimeError("torch.ops.mgx.rotary forms no tangent: use musicgeneration_amd.ops.rotary")
     return ops._rotary(x, ops._dense_like(x), cos, sin, positions, half, 1 if transposed else 0)
 
 
