@@ -1189,6 +1189,11 @@ def _beside(t, name, like, dtypes):
         raise ValueError(f"{name} must be contiguous")
 
 
+def _written(*ts):
+    """Tells autograd that a kernel has written ts in place: a backward that saved one of them raises."""
+    torch.autograd.graph.increment_version(ts)
+
+
 _FP32, _INT32, _INTS = (torch.float32,), (torch.int32,), (torch.int32, torch.int64)
 
 
@@ -1348,7 +1353,9 @@ def rotary_(x, cos, sin, positions=None, layout: str = "interleaved", transposed
         raise RuntimeError("rotary_ turns no tangent: use rotary")
     if _overlaps(x):
         raise ValueError("rotary_: elements of x share memory")
-    return _rotary(x, x, cos, sin, positions, half, 1 if transposed else 0)
+    _rotary(x, x, cos, sin, positions, half, 1 if transposed else 0)
+    _written(x)
+    return x
 
 
 # ---------------------------------------------------------------------------
@@ -1430,6 +1437,7 @@ def paged_append(qkv, kcache, vcache, table, lens, n_heads: int, cos=None, sin=N
             qkv.data_ptr(), q_ptr, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows),
             _p(cos), _p(sin), T, B, 0 if cu_rows is not None else lead[1], n_heads, Hkv, dh, rd, page, n_pages, width, rows,
             offset, _HALF[layout], _DT[qkv.dtype])), "mgx_paged_append")
+        _written(kcache, vcache)
     return q
 
 

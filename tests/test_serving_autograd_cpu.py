@@ -67,3 +67,21 @@ def test_what_forms_no_tangent_refuses_one(launches):
         refuse(ops.verify_draft, _dual(p), x, u, d)
         refuse(ops.verify_draft, p, x, u, _dual(d))
     assert not launches
+
+
+def test_writes_in_place_raise_the_version(launches):
+    """What an earlier operation saved for its backward must not be taken for the values it saw."""
+    x, c = E(2, 5, 3, 16), E(8, 4)
+    before = x._version
+    ops.rotary_(x[:, 1:], c, c)
+    assert x._version > before
+    qkv, cache = E(3, 2, 8 * 64, dtype=BF16), _cache()
+    for tables in ({}, {"cos": E(9, 32), "sin": E(9, 32)}):
+        before = {n: t._version for n, t in {**cache, "qkv": qkv}.items()}
+        ops.paged_append(qkv, **cache, n_heads=4, **tables)
+        after = {n: t._version for n, t in {**cache, "qkv": qkv}.items()}
+        assert {n for n in after if after[n] > before[n]} == {"kcache", "vcache"}
+    q = E(3, 2, 4, 64, dtype=BF16)
+    before = {n: t._version for n, t in {**cache, "q": q}.items()}
+    ops.paged_attn(q, **cache)
+    assert before == {n: t._version for n, t in {**cache, "q": q}.items()}

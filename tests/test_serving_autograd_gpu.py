@@ -55,3 +55,26 @@ def test_dispatched_operators_refuse_tangents():
         p = torch.rand(1, 3, 9, device="cuda")
         with pytest.raises(RuntimeError, match="tangent"):
             torch.ops.mgx.verify_draft(fwd.make_dual(p, p), torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.rand(1, 3, device="cuda"))
+
+
+def test_a_backward_that_saved_what_was_written_over_raises():
+    from musicgeneration_amd import ops
+    cos, sin = ops.rope_tables(40, 64)
+    w = torch.randn(64, device="cuda").requires_grad_()
+    x = torch.randn(1, 4, 2, 64, device="cuda")
+    z = w * x
+    ops.rotary_(x, cos, sin)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    kc, vc = (torch.zeros(3, 2, 16, 64, device="cuda") for _ in range(2))
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda")
+    for which in (kc, vc):
+        z = w * which
+        ops.paged_append(torch.randn(1, 4, 6 * 64, device="cuda"), kc, vc, table, lens, 2, cos, sin)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+    # tensors made in inference mode have no counter
+    with torch.inference_mode():
+        y = torch.randn(1, 4, 2, 64, device="cuda")
+        want = ops.rotary(y, cos, sin)
+        assert torch.equal(ops.rotary_(y, cos, sin), want)
