@@ -408,6 +408,10 @@ int mgx_paged_append(const void* qkv, void* q_out, void* kcache, void* vcache, c
  * workspace: mgx_paged_attn_workspace_floats floats for the same arguments.  dh <= 256, a multiple of 16 bytes. */
 long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows, int max_len,
                                      int dtype);
+/* How mgx_paged_attn takes a call of these sizes apart (host only): plan[0] whether the prefix has items of its own, [1] and
+ * [2] the tiles of prefix and of own items (0: 16 rows of a workgroup, 1: 32, 2: 128, 3: 256, 4: 16 rows on eight waves), [3]
+ * and [4] into how many ranges the prefix's and the own keys go at most, [5] and [6] the keys of one range. */
+int mgx_paged_attn_plan(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows, int max_len, int dtype, int* plan);
 int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const void* vcache, const int* table,
                    const int* lens, const int* cu_rows, const float* slopes, const int* prefix, void* out, float* workspace,
                    long T, int B, int R, int Hq, int Hkv, int dh, int page, int n_pages, int width, int prefix_len,

@@ -75,6 +75,7 @@ PROTOTYPES = {
     "mgx_rope_tables": (_i, [_vp, _vp, _vp, _l, _i, _d, _vp]),
     "mgx_paged_append": (_i, [_vp] * 9 + [_l] + [_i] * 13 + [_vp]),
     "mgx_paged_attn_workspace_floats": (_l, [_l] + [_i] * 8),
+    "mgx_paged_attn_plan": (_i, [_l] + [_i] * 8 + [C.POINTER(C.c_int)]),
     "mgx_paged_attn": (_i, [_vp, _l] + [_vp] * 9 + [_l] + [_i] * 11 + [_f, _i, _vp]),
     "mgx_verify_draft": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _l, _l, _l, _l, _l, _i, _vp]),
     "mgx_gemm_tn_pair_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp]),

@@ -1244,6 +1244,19 @@ extern "C" long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, 
     return (p.So + p.Sp) * T * Hq * (dh + 2L);
 }
 
+extern "C" int mgx_paged_attn_plan(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows, int max_len, int dtype,
+                                   int* plan) {
+    MGX_REQUIRE(plan, MGX_EINVAL, "mgx_paged_attn_plan: null pointer");
+    MGX_REQUIRE(T > 0 && B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && dh > 0 && dh <= 256 && max_rows > 0 && max_len > 0 &&
+                    prefix_len >= 0 && (dtype == MGX_F32 || dtype == MGX_BF16),
+                MGX_EINVAL, "mgx_paged_attn_plan: T=%ld B=%d Hq=%d Hkv=%d dh=%d prefix=%d max_rows=%d max_len=%d dtype=%d", T, B, Hq,
+                Hkv, dh, prefix_len, max_rows, max_len, dtype);
+    const Plan p = plan_of(T, B, Hq, Hkv, dh, prefix_len, max_rows, max_len, dtype);
+    const int out[7] = {p.share, p.body_p, p.body_o, p.Sp, p.So, p.chunk_p, p.chunk_o};
+    for (int i = 0; i < 7; ++i) plan[i] = out[i];
+    return MGX_OK;
+}
+
 extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcache, const void* vcache, const int* table,
                               const int* lens, const int* cu_rows, const float* slopes, const int* prefix, void* out,
                               float* workspace, long T, int B, int R, int Hq, int Hkv, int dh, int page, int n_pages,
