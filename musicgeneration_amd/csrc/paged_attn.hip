@@ -499,14 +499,15 @@ struct Rows {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x = fmaxf(x, s[i][tb][r]);
             mx[i] = half_swap_max(x);
-            grown |= !((mx[i] - m[i]) * c <= RESCALE_LOG2);
+            grown |= (mx[i] - m[i]) * c > RESCALE_LOG2;
         }
-        // the stale maximum stays while no row's grew by more than 2^8: weights are then at most 2^8, which fp32 sums and
-        // bf16 weights hold with the same relative precision
+        // A row's stale maximum stays until it has grown by more than 2^8: weights are then at most 2^8, which fp32 sums and
+        // bf16 weights hold with the same relative precision.  Each row for itself: what another row of the wave holds (NaN,
+        // infinities) does not change its result.
         if (__any(grown)) {
 #pragma unroll
             for (int i = 0; i < RW; ++i) {
-                const float mn = fmaxf(m[i], mx[i]);
+                const float mn = (mx[i] - m[i]) * c > RESCALE_LOG2 ? mx[i] : m[i];
                 const float alpha = fast_exp2((m[i] - mn) * c);
                 m[i] = mn;
                 l[i] *= alpha;
@@ -610,12 +611,12 @@ struct Rows16 {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x = fmaxf(x, s[rt][kt][r]);
             mx[rt] = quarter_max(x);
-            grown |= !((mx[rt] - m[rt]) * c <= RESCALE_LOG2);
+            grown |= (mx[rt] - m[rt]) * c > RESCALE_LOG2;
         }
         if (__any(grown)) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float mn = fmaxf(m[rt], mx[rt]);
+                const float mn = (mx[rt] - m[rt]) * c > RESCALE_LOG2 ? mx[rt] : m[rt];      // (see Rows::take)
                 const float alpha = fast_exp2((m[rt] - mn) * c);
                 m[rt] = mn;
                 l[rt] *= alpha;

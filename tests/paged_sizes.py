@@ -55,3 +55,11 @@ def plan_of_case(case, ragged, spare=3):
     dtype, dh, _, _, _, B, R, Hq, Hkv, P, longest = case
     T = sum(rows_of_sequences(B, R, ragged)) + (spare if ragged else 0)
     return plan(T, B, Hq, Hkv, dh, P, R, longest, dtype)
+
+
+# (sequences, rows, Hq, Hkv, longest own length): prompts whose rows fill several tiles, over several tiles of keys
+PROMPTS = [(2, 150, 2, 1, 400), (40, 130, 2, 1, 300), (60, 130, 2, 2, 400)]
+# (dtype, dh) -> [(sequences, rows, Hq, Hkv, prefix, longest own length)]: prefix items of many sequences' rows, several tiles of keys each
+NEIGHBOURS = {(dtype, dh): [(64, 1, 8, 8, 2050, 700), (150, 1, 8, 4, 2050, 700), (30, 33, 8, 8, 2050, 133)] for dtype in (F32, BF16) for dh in (64, 128, 256)}
+for _at in ((F32, 64), (BF16, 64), (BF16, 128), (F32, 256)):
+    NEIGHBOURS[_at].append((48, 6, 16, 4, 2050, 106))

@@ -1,14 +1,17 @@
 """Every form of paged_attn's kernel (private and shared tiles, prefix taken apart or not, ranges split or whole) against the 64-bit
 loop, at sizes of which tests/test_paged_plan_cpu.py asserts that they reach it."""
+import math
+
 import pytest
 import torch
 
-from paged_sizes import ALL, NAMES, rows_of_sequences
+from paged_sizes import ALL, BF16, F32, NAMES, NEIGHBOURS, PROMPTS, rows_of_sequences
 from serving_oracle import assert_attended, attend
 from test_paged_gpu import _pool
 
 pytestmark = pytest.mark.gpu
 SPARE = 3
+NAN = float("nan")
 
 
 def _inputs(case, ragged, seed=0, size=1.0):
@@ -49,3 +52,61 @@ def test_every_form(case, ragged):
         assert_attended(got, want, bound)
         if ragged:
             assert not got[cu[-1]:].any()
+
+
+def _bits(x):
+    """x as whole numbers: equal bit for bit, NaN too."""
+    return x.view(torch.int16 if x.dtype is BF16 else torch.int32)
+
+
+@pytest.mark.parametrize("dtype,dh", list(NEIGHBOURS))
+@pytest.mark.parametrize("size", PROMPTS, ids=str)
+def test_prompts_see_no_value_behind_their_row(dtype, dh, size):
+    """Infinities and NaN in the v (and NaN in the k) of rows of the same prompt, in the first, a middle and the last tile and in several
+    at once: earlier rows stay the same, bit for bit; later ones are not finite in the v's channel alone, or anywhere where k is bad."""
+    B, R, Hq, Hkv, longest = size
+    case = (dtype, dh, 0, 0, 0, B, R, Hq, Hkv, 0, longest)
+    q, k, v, table, lens, _, prefix = _inputs(case, False, seed=dh + B, size=4.0)
+    clean = _call(case, q, k, v, table, lens, None, prefix).cpu()
+    others = [d for d in range(dh) if d != 5]
+    for rows, bad, in_k in (((0,), NAN, False), ((R // 2,), math.inf, False), ((R - 1,), -math.inf, False), ((3, R // 2, R - 2), math.inf, False),
+                            ((1,), NAN, True), ((R // 2 + 1, R - 1), NAN, True)):
+        k2, v2 = k.clone(), v.clone()
+        for b, n in enumerate(lens):
+            for row in rows:
+                j = n - R + row
+                (k2 if in_k else v2)[table[b, j // 16], :, j % 16, 5] = bad
+        got = _call(case, q, k2, v2, table, lens, None, prefix).cpu()
+        first = rows[0]
+        assert torch.equal(_bits(got[:, :first]), _bits(clean[:, :first])), (rows, bad, in_k)
+        if in_k:
+            assert torch.isnan(got[:, first:]).all(), (rows, bad)
+        else:
+            assert not torch.isfinite(got[:, first:, :, 5].float()).any(), (rows, bad)
+            assert torch.equal(_bits(got[..., others]), _bits(clean[..., others])), (rows, bad)
+
+
+def _rows_stay_alone(case, seed):
+    dtype, dh, B, R = case[0], case[1], case[5], case[6]
+    q, k, v, table, lens, _, prefix = _inputs(case, False, seed=seed, size=4.0)
+    clean = _call(case, q, k, v, table, lens, None, prefix)
+    q[1], q[B - 1, 0] = NAN, math.inf
+    got = _call(case, q, k, v, table, lens, None, prefix)
+    stay = torch.ones(B, R, dtype=torch.bool)
+    stay[1], stay[B - 1, 0] = False, False
+    stay = stay.cuda()
+    assert torch.equal(_bits(got[stay]), _bits(clean[stay]))
+    assert not torch.isfinite(got[~stay].float()).any()
+
+
+@pytest.mark.parametrize("case", [(*at, 1, 0, 0, *size) for at, sizes in NEIGHBOURS.items() for size in sizes], ids=str)
+def test_a_row_that_is_not_a_number_leaves_its_neighbours_in_a_tile_alone(case):
+    """The tiles of a prefix hold rows of many sequences (a padded batch: some are NaN or infinite): the others stay the same, bit for
+    bit, over many tiles of keys, where the running maxima move."""
+    _rows_stay_alone(case, 7)
+
+
+@pytest.mark.parametrize("dtype,dh", list(NEIGHBOURS))
+@pytest.mark.parametrize("size", PROMPTS, ids=str)
+def test_a_row_of_a_prompt_that_is_not_a_number_leaves_the_others_alone(dtype, dh, size):
+    _rows_stay_alone((dtype, dh, 0, 0, 0, *size[:4], 0, size[4]), 8)

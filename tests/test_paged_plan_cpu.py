@@ -4,7 +4,7 @@ import ctypes
 
 import pytest
 
-from paged_sizes import ALL, BF16, F32, NAMES, SIZES, plan_of_case
+from paged_sizes import ALL, BF16, F32, NAMES, NEIGHBOURS, PROMPTS, SIZES, plan, plan_of_case
 
 # every form the launcher has an instance of: (dtype, dh) -> {(share, tiles of prefix items, of own items)}
 FORMS = {
@@ -37,6 +37,23 @@ def test_every_form_is_reached_with_whole_and_split_ranges():
         assert any(p["share"] and p["chunk_p"] == 64 for c, p in plans if c[0] is dtype)
         assert any(p["share"] and p["body_p"] >= 2 and p["chunk_p"] > 64 for c, p in plans if c[0] is dtype)
     assert any(p["share"] and p["body_p"] == 2 and p["chunk_p"] >= 512 for c, p in plans) and any(p["share"] and p["body_p"] == 3 and p["chunk_p"] >= 512 for c, p in plans)
+
+
+def test_prompts_and_neighbours_fill_tiles():
+    own, prefix = {}, {}
+    for at, sizes in NEIGHBOURS.items():
+        for B, R, Hq, Hkv, longest in PROMPTS:
+            p = plan(B * R, B, Hq, Hkv, at[1], 0, R, longest, at[0])
+            own.setdefault((*at, p["body_o"]), set()).add(p["So"] > 1)
+        for B, R, Hq, Hkv, P, longest in sizes:
+            p = plan(B * R, B, Hq, Hkv, at[1], P, R, longest, at[0])
+            assert p["share"] and p["chunk_p"] >= 192, (at, B, R, p)
+            prefix.setdefault(at, set()).add((p["body_p"], p["body_o"]))
+    # shared tiles of every kind, with whole and with split ranges
+    assert all(own[at] == {False, True} for at in ((F32, 64, 2), (F32, 128, 2), (BF16, 128, 2), (BF16, 64, 3), (BF16, 256, 2))), own
+    assert (BF16, 64, 2) in own and (F32, 256, 0) in own
+    assert prefix == {(F32, 64): {(2, 0), (2, 1), (2, 2)}, (F32, 128): {(2, 0), (2, 2)}, (F32, 256): {(0, 0)}, (BF16, 64): {(2, 0), (3, 0), (3, 1), (3, 3)},
+                      (BF16, 128): {(2, 0), (2, 1), (2, 2)}, (BF16, 256): {(0, 0)}}
 
 
 def test_plan_refuses():
