@@ -110,3 +110,18 @@ def test_a_row_that_is_not_a_number_leaves_its_neighbours_in_a_tile_alone(case):
 @pytest.mark.parametrize("size", PROMPTS, ids=str)
 def test_a_row_of_a_prompt_that_is_not_a_number_leaves_the_others_alone(dtype, dh, size):
     _rows_stay_alone((dtype, dh, 0, 0, 0, *size[:4], 0, size[4]), 8)
+
+
+PRIVATE = [c for c in ALL if c[0] is BF16 and (c[3] in (0, 1) or not c[2]) and c[4] in (0, 1, 4)]
+
+
+@pytest.mark.parametrize("case", PRIVATE, ids=str)
+def test_private_tiles_keep_the_weights_precise(case):
+    """bf16 calls of few rows: the weights enter the product with V as a bf16 value and the bf16 rounding of what it leaves, which is at
+    most 2^-7 of it: off by 2^-8 x 2^-7 (and the 2^-24 that the remainder is raised by), where `attend` allows two roundings of 2^-8."""
+    q, k, v, table, lens, cu, prefix = _inputs(case, False, seed=3)
+    args = (table, lens, None, cu, prefix if case[9] else None, case[9])
+    want, bound = attend(q, k, v, *args)
+    weighed, _ = attend(q, k, v.abs(), *args)             # sum_j p_j |v_j|
+    got = _call(case, q, k, v, table, lens, cu, prefix)
+    assert_attended(got, want, bound - (2 * 2.0 ** -8 - 2.0 ** -15 - 2.0 ** -23) * weighed)
