@@ -541,7 +541,8 @@ struct Rows {
         }
         pr.template weigh<NB, RW>(V, va, s, o, l);
     }
-    // Keys j0 .. j0+31, whose V values that are not finite were left out: rows that see such a key get NaN there.
+    // Keys j0 .. j0+31, whose V values that are not finite were left out: rows that see such a key have them added (an infinity
+    // times a weight is the infinity).
     __device__ __forceinline__ void spoil(const PagedArgs& a, const int* own, int hk, int j0, int end, int h5) {
         for (int j = j0; j < min(j0 + 32, end); ++j) {
             const unsigned kr = slot_of(a, hk, page_of(a, own, j, end), j, end);
@@ -552,10 +553,11 @@ struct Rows {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int at_d = 32 * d + 8 * (r >> 2) + 4 * h5 + (r & 3);
-                    const bool bad = at_d < a.dh && !(fabsf(to_f32(v[at_d])) < INFINITY);
+                    const float x = at_d < a.dh ? to_f32(v[at_d]) : 0.f;
+                    const bool bad = !(fabsf(x) < INFINITY);
 #pragma unroll
                     for (int i = 0; i < RW; ++i)
-                        if (bad && j <= limit[i]) o[i][d][r] = __builtin_nanf("");
+                        if (bad && j <= limit[i]) o[i][d][r] += x;
                 }
         }
     }
@@ -665,10 +667,11 @@ struct Rows16 {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int at_d = 16 * d + 4 * g + r;
-                    const bool bad = at_d < a.dh && !(fabsf(to_f32(v[at_d])) < INFINITY);
+                    const float x = at_d < a.dh ? to_f32(v[at_d]) : 0.f;
+                    const bool bad = !(fabsf(x) < INFINITY);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        if (bad && j <= limit[rt]) o[rt][d][r] = __builtin_nanf("");
+                        if (bad && j <= limit[rt]) o[rt][d][r] += x;
                 }
         }
     }

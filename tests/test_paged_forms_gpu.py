@@ -125,3 +125,32 @@ def test_private_tiles_keep_the_weights_precise(case):
     weighed, _ = attend(q, k, v.abs(), *args)             # sum_j p_j |v_j|
     got = _call(case, q, k, v, table, lens, cu, prefix)
     assert_attended(got, want, bound - (2 * 2.0 ** -8 - 2.0 ** -15 - 2.0 ** -23) * weighed)
+
+
+@pytest.mark.parametrize("dtype,dh", list(NEIGHBOURS))
+@pytest.mark.parametrize("B,R", [(3, 1), (2, 20), (2, 150)])
+def test_infinite_values_come_out_infinite(dtype, dh, B, R):
+    """out = sum_j p_j v_j, p_j > 0: where a row sees one infinite v, wherever in a tile it lies, that is the result; where it sees
+    infinities of both signs or a NaN, NaN.  (Weights far from underflow: |scores| < 10.)"""
+    from musicgeneration_amd import ops
+    n, page = 330, 16
+    k, v, table, _, g = _pool([n] * B, 1, page, dh, dtype, seed=dh)
+    q = torch.randn(B, R, 2, dh, generator=g).to(dtype)
+    last = n - R                                          # own index of the first row
+    keys = {1: (0, math.inf), 2: (last, -math.inf), 3: (n - 1, math.inf), 4: (last - 40, math.inf), 6: (last + R // 2, NAN)}
+    for channel, (j, bad) in keys.items():
+        for b in range(B):
+            v[table[b, j // page], :, j % page, channel] = bad
+    for b in range(B):                                    # channel 7: both signs, the second from row R / 2 on
+        v[table[b, 2 // page], :, 2 % page, 7] = math.inf
+        j = last + R // 2
+        v[table[b, j // page], :, j % page, 7] = -math.inf
+    got = ops.paged_attn(q.cuda(), k.cuda(), v.cuda(), table.cuda(), torch.full((B,), n, dtype=torch.int32).cuda()).float().cpu()
+    sees = torch.arange(R)[None, :, None].expand(B, R, 2) + last      # last key of a row
+    for channel, (j, bad) in keys.items():
+        x, seen = got[..., channel], sees >= j
+        assert torch.isfinite(x[~seen]).all(), channel
+        assert torch.isnan(x[seen]).all() if bad != bad else (x[seen] == bad).all(), channel
+    both = sees >= last + R // 2
+    assert torch.isnan(got[..., 7][both]).all() and (got[..., 7][~both] == math.inf).all()
+    assert torch.isfinite(got[..., [0, 5]]).all()
