@@ -1381,7 +1381,7 @@ def _cache_args(kcache, vcache, table, lens, like, name):
         raise ValueError(f"{name}: head dim {dh} must be a multiple of {16 // kcache.element_size()} up to 256")
     _beside(table, "table", like, _INT32)
     _beside(lens, "lens", like, _INT32)
-    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0] or table.numel() == 0:
+    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0] or table.shape[1] == 0:
         raise ValueError(f"{name}: table {tuple(table.shape)} must be [sequences, pages], lens {tuple(lens.shape)} [sequences]")
     return n_pages, Hkv, page, dh
 
@@ -1432,6 +1432,8 @@ def paged_append(qkv, kcache, vcache, table, lens, n_heads: int, cos=None, sin=N
         _rope_tables_ok(cos, sin, dh, qkv, name)
         q = qkv.new_empty((*lead, n_heads, dh))
         q_ptr, rows, rd = q.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+    if T and not B:                               # rows of no sequence
+        return q if cos is None else q.zero_()
     if T:
         check(_on(qkv.device, lib.mgx_paged_append, (
             qkv.data_ptr(), q_ptr, kcache.data_ptr(), vcache.data_ptr(), table.data_ptr(), lens.data_ptr(), _p(cu_rows),
@@ -1484,8 +1486,8 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
         raise ValueError(f"{name}: scale {scale}")
     out = _dense_like(q)
     T = out.numel() // (Hq * dh)
-    if T == 0:
-        return out
+    if T == 0 or B == 0:
+        return out.zero_()
     if T * Hq >= 2 ** 30:
         raise ValueError(f"{name}: {T} rows of {Hq} heads")
     R = 0 if cu_rows is not None else q.shape[1]
