@@ -405,7 +405,7 @@ int mgx_paged_append(const void* qkv, void* q_out, void* kcache, void* vcache, c
  * q [T,Hq,dh] with q_row_stride elements from row to row, out [T,Hq,dh]; query head h reads K/V head h / (Hq / Hkv).
  * A row that sees no key, and a row of no sequence, gets zeros.  What masked slots hold (stale values, NaN) has no
  * effect.  max_rows / max_len: upper bounds of n_b and lens[b] that shape the launch (wrong ones cost time, not results).
- * workspace: mgx_paged_attn_workspace_floats floats for the same arguments.  dh <= 256, a multiple of 16 bytes. */
+ * workspace: mgx_paged_attn_workspace_floats floats for the same arguments.  dh <= 256, a multiple of 16 bytes; |scale| < 2^127. */
 long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows, int max_len,
                                      int dtype);
 /* How mgx_paged_attn takes a call of these sizes apart (host only): plan[0] whether the prefix has items of its own, [1] and

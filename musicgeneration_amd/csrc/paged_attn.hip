@@ -1288,6 +1288,7 @@ extern "C" int mgx_paged_attn(const void* q, long q_row_stride, const void* kcac
     MGX_REQUIRE(prefix_len >= 0 && (prefix || prefix_len == 0), MGX_EINVAL, "mgx_paged_attn: prefix of %d keys", prefix_len);
     MGX_REQUIRE((long)page * width + prefix_len < (1L << 30), MGX_EUNSUPPORTED, "mgx_paged_attn: more than 2^30 keys");
     MGX_REQUIRE(max_rows > 0 && max_len > 0, MGX_EINVAL, "mgx_paged_attn: max_rows=%d max_len=%d", max_rows, max_len);
+    MGX_REQUIRE(fabsf(scale) < 0x1p127f, MGX_EINVAL, "mgx_paged_attn: scale %g", scale);        // (times log2 e: an fp32 number)
     MGX_REQUIRE(dtype == MGX_F32 || dtype == MGX_BF16, MGX_EINVAL, "mgx_paged_attn: bad dtype %d", dtype);
     const int N = dtype == MGX_F32 ? 4 : 8;
     MGX_REQUIRE(dh % N == 0 && dh <= 256, MGX_EUNSUPPORTED, "mgx_paged_attn: head dim %d must be a multiple of %d up to 256", dh, N);

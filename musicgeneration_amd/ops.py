@@ -1482,7 +1482,7 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     if page * width + prefix_len >= 2 ** 30:
         raise ValueError(f"{name}: tables of {page * width} keys behind {prefix_len}")
     scale = dh ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) < 2.0 ** 127:                # (times log2 e it has to be an fp32 number)
         raise ValueError(f"{name}: scale {scale}")
     out = _dense_like(q)
     T = out.numel() // (Hq * dh)

@@ -47,3 +47,22 @@ def test_empty_batches_need_no_launch(launches):
     assert not launches
     with pytest.raises(ValueError, match="table"):
         ops.paged_attn(E(0, 2, 4, 64, dtype=BF16), **{**cache, "table": E(0, 0, dtype=I32)})
+
+
+def test_scales_that_fp32_does_not_hold_are_refused(launches):
+    """The kernel works in fp32, with the scale times log2 e: beyond 2^127 there would be NaN."""
+    cache, q = _cache(3), E(3, 2, 4, 64, dtype=BF16)
+    for scale in (2.0 ** 127, -1e39, 1e300, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            ops.paged_attn(q, **cache, scale=scale)
+    assert not launches
+    for scale in (1e38, -1e38, 0.0, 1e-300):
+        ops.paged_attn(q, **cache, scale=scale)
+    assert len(launches) == 4
+
+
+def test_c_entry_point_refuses_such_scales():
+    a, b, n = 16, 32, None
+    for scale in (2.0 ** 127, -2.0 ** 127, math.inf, -math.inf, math.nan):
+        assert lib.mgx_paged_attn(a, 8, a, b, a, a, n, n, n, a, a, 2, 2, 1, 1, 1, 8, 4, 2, 2, 0, 1, 8, scale, 1, n) == -1
+        assert b"scale" in lib.mgx_last_error_string()
