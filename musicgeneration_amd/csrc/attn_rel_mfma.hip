@@ -94,9 +94,9 @@ template <int DH>
 __device__ __forceinline__ void load_er_rows(bf16x8 (&ef)[DH / 16], const bf16_t* Eh, int M, int Rb, int l31, int h5) {
     int idx = M - 1 - (Rb + l31);
     idx = min(max(idx, 0), M - 1);
-    const bf16_t* p = Eh + (long)idx * DH + 8 * h5;
+    const unsigned at = (unsigned)idx * DH + 8u * h5;
 #pragma unroll
-    for (int ks = 0; ks < DH / 16; ++ks) ef[ks] = *reinterpret_cast<const bf16x8*>(p + 16 * ks);
+    for (int ks = 0; ks < DH / 16; ++ks) ef[ks] = *reinterpret_cast<const bf16x8*>(Eh + (at + 16u * ks));
 }
 
 // ---- Er as a third tile stream (query-on-lane kernels) ---------------------------------------------------------
@@ -583,22 +583,20 @@ __global__ __launch_bounds__(64 * NW, (DH == 128 ? 1 : 2)) void rel_bwd_dkv_mfma
     const int t0 = jb0 / 64;
     const int ntiles = (S + 63) / 64;
     TileRegs<DH, NT> qr, gr;
-    float r_lse = 0.f, r_delta = 0.f;
+    // wave 0: lse, wave 1: delta.  One register, as 256 are tight: values spilled in the loop are reloaded behind the tile's
+    // loads in flight and wait for those, too (17 spilled: 660 us at B8 S4096, 3, none of them per block: 525)
+    float r_stat = 0.f;
     auto load_tile = [&](int i0) {
         tile_load<DH, NT>(qr, base, rs, i0, S, tid);
         tile_load<DH, NT>(gr, gp, (unsigned)(H * DH), i0, S, tid);
-        if (tid < 64 && i0 + tid < S) {
-            r_lse = lse_bh[i0 + tid];
-            r_delta = delta_bh[i0 + tid];
-        }
+        if (w < 2 && i0 + lane < S) r_stat = (w ? delta_bh : lse_bh)[i0 + lane];
     };
     auto store_tile = [&](int i0, int buf) {
         tile_store<DH, NT>(qr, smem + buf * 2 * TB, tid);
         tile_store<DH, NT>(gr, smem + buf * 2 * TB + TB, tid);
-        if (tid < 64) {
-            const bool ok = i0 + tid < S;
-            stats[buf * 128 + tid] = ok ? -(r_lse * LOG2E * inv_c) : -INFINITY;
-            stats[buf * 128 + 64 + tid] = ok ? -r_delta : 0.f;
+        if (w < 2) {
+            const bool ok = i0 + lane < S;
+            stats[buf * 128 + tid] = w ? (ok ? -r_stat : 0.f) : ok ? -(r_stat * LOG2E * inv_c) : -INFINITY;
         }
     };
     load_tile(t0 * 64);
