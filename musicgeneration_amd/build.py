@@ -41,7 +41,7 @@ def build(force=False, verbose=True):
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ, src[:-4] + ".o")
         objs.append(o)
-        if force or _stale(o, [s] + headers):
+        if force or _stale(o, [s, __file__] + headers):            # (this file holds the flags)
             jobs.append([HIPCC, *FLAGS, "-c", s, "-o", o])
 
     def run(cmd):
