@@ -404,7 +404,9 @@ int mgx_paged_append(const void* qkv, void* q_out, void* kcache, void* vcache, c
  *   out = softmax(scale q.k + slope_h (j - i)) v      i = prefix_len + own index; slopes [Hq] fp32 or NULL
  * q [T,Hq,dh] with q_row_stride elements from row to row, out [T,Hq,dh]; query head h reads K/V head h / (Hq / Hkv).
  * A row that sees no key, and a row of no sequence, gets zeros.  What masked slots hold (stale values, NaN) has no
- * effect.  max_rows / max_len: upper bounds of n_b and lens[b] that shape the launch (wrong ones cost time, not results).
+ * effect.  max_rows / max_len: upper bounds of n_b and lens[b] that shape the launch (wrong ones cost time, not results beyond
+ * their last bits).  Softmax, sums and joins in fp32; bf16 weights enter the product with v in two bf16 parts in private tiles,
+ * rounded to bf16 in shared ones (mgx_paged_attn_plan).
  * workspace: mgx_paged_attn_workspace_floats floats for the same arguments.  dh <= 256, a multiple of 16 bytes; |scale| < 2^127. */
 long mgx_paged_attn_workspace_floats(long T, int B, int Hq, int Hkv, int dh, int prefix_len, int max_rows, int max_len,
                                      int dtype);

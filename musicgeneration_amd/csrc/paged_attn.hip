@@ -20,18 +20,25 @@
 //            four waves.
 // Ranges of one row are joined by a second kernel from unnormalised fp32 sums with their maxima (fixed order).
 //
-// Measured (library product of 8192^3 bf16: 1172 TFLOP/s; copy: 5.15 TB/s; calls one after another):
-//   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     50 us   (own keys alone 36: 3.8 TB/s; prefix alone
+// bf16 weights: the private tiles take them into the product with V in two bf16 parts (15 bits or more); the shared tiles round
+// them to bf16, and divide by the sum of the rounded ones.  Two parts there were measured: 128 x 6 rows behind 16385 keys 139
+// -> 181 us, the prompts 378 -> 488, so they keep the rounding of the training attention (attn_mfma.hip).
+//
+// Measured (library product of 8192^3 bf16: 1172 TFLOP/s; copy: 5.15 TB/s; graph replays of calls one after another):
+//   64 sequences x 1 row, 32 + 8 heads of 128, prefix 8192, own <= 1024     52 us   (own keys alone 36: 3.7 TB/s; prefix alone
 //                                                                           32; together they overlap in part)
-//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   122 us  560 TFLOP/s (143 us without a pause between
-//                                                                           calls): a SIMD issues in 70 % of its busy cycles,
-//                                                                           its matrix unit works in 28 %
-//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        352 us  727 TFLOP/s (381 without a pause): issue
-//                                                                           56 %, matrix unit 31 %, neither full
-//   16 sequences x 1 row, 8 heads of 64, own <= 2048                        14 us of kernel (one key each instead: 6 to 7)
+//   128 sequences x 6 rows, 20 + 4 heads of 64, prefix 16385, own <= 2006   143 us  479 TFLOP/s (137 to 154 from box to box and run
+//                                                                           to run): a SIMD issues in 70 % of its busy cycles, its
+//                                                                           matrix unit works in 29 %; 1.65 waves a SIMD
+//   9 prompts of 1..1500 rows, 16 + 2 heads of 128, behind 4001 keys        381 us  673 TFLOP/s: issue 56 %, matrix unit 31 %; 1.51
+//                                                                           waves a SIMD (852 row tiles on 512 slots: the second
+//                                                                           round leaves slots empty)
+//   1 prompt of 4096 / 8192 rows, 32 + 8 heads of 128, no prefix            228 / 709 us  604 / 776 TFLOP/s
+//   16 sequences x 1 row, 8 heads of 64, own <= 2048                        14.5 us of kernel, 16 a call (one key each instead: 6 to 7)
 //   1 sequence, 8 heads of 128, 30001 keys                                  36 us   (3.4 TB/s with the join)
-//   16 sequences x 1 row, 8 heads of 256, own <= 2048                       36 us   (3.7 TB/s)
-//   9 prompts of 1..1500 rows, 16 + 2 heads of 256, behind 4001 keys        1.06 ms 480 TFLOP/s
+//   16 sequences x 1 row, 8 heads of 256, own <= 2048                       43 us   (3.1 TB/s)
+//   9 prompts of 1..1500 rows, 16 + 2 heads of 256, behind 4001 keys        1.04 to 1.12 ms 458 TFLOP/s
+//   the prompts in fp32, heads of 128 / 64                                  3.08 / 1.44 ms  83 / 89 TFLOP/s (library product 154)
 //   24 x 3 rows fp32, 12 + 4 heads of 64, prefix 1000, own <= 703           16 + 4 us: latency
 // A launch whose items hold one key takes 5.6 us (1 sequence) to 8 us (64, heads of 128): the beginning (length, page, keys:
 // three dependent loads) and the end of an item.  That is what limits splitting; the plan reckons 5 us an item.
@@ -145,8 +152,8 @@ template <int DH> struct Prod<bf16_t, DH> {       // v_mfma_f32_32x32x16_bf16; i
         for (int d = 0; d < DH / 32; ++d) v.f[d] = lds_read_tr_pair(V + la.tr_read(tb, s2, 0, d), V + la.tr_read(tb, s2, 1, d));
         return v;
     }
-    // P is rounded to bf16 for the product (2^-8 relative each, signs independent) and so for the sum, so that the weights
-    // add up to one; two values an instruction
+    // P is rounded to bf16 for the product (2^-8 relative each, signs independent; two parts cost a third of the time, see
+    // above) and so for the sum, so that the weights add up to one; two values an instruction
     template <int NB, int RW>
     __device__ __forceinline__ void weigh(const char* V, VAhead now, const f32x16 (&p)[RW][NB], f32x16 (&o)[RW][DH / 32],
                                           float (&l)[RW]) const {

@@ -11,7 +11,8 @@
 // take consecutive units, then head groups, so a wave's request covers whole heads (128 bytes and more).
 // Measured (a copy of 1 GiB moves 5.15 TB/s): q | k heads of 16 x 2048 rows, 16 heads of 64, bf16: 26 us = 5.1 TB/s;
 // prompts of 16.5 k rows, 32 + 2 x 8 heads of 128, rotated and filed: 78.7 us = 5.15 TB/s; one row for each of 64 sequences:
-// 4.5 us, of which the launch, two dependent loads (length, page) and the row's own are nearly all.
+// 4.5 us, of which the launch, two dependent loads (length, page) and the row's own are nearly all.  Sizes off the 16-byte
+// grid (bf16, half layout, 40 of 80 values turned) take units of one value: 1.8 TB/s, rotated or filed (32 of 80: 3.8).
 #include "mgx_common.h"
 
 namespace {

@@ -1220,7 +1220,8 @@ def rope_tables(n: int, rotary_dim: int, base: float = 10000.0, scaling=None, fa
       "linear"    theta_i / factor (positions interpolated)
       "ntk"       base * factor^(rd/(rd-2)): the slowest pair is interpolated by `factor`, the fastest not at all
       "by_parts"  pairs that turn more than 32 times over the `original` trained length stay, those that turn less than
-                  once are interpolated, a linear ramp between; cos and sin are scaled by 1 + 0.1 ln(factor)
+                  once are interpolated, a linear ramp between; cos and sin are scaled by 1 + 0.1 ln(factor): the YaRN
+                  method (Peng et al., 2023) with its published constants
     """
     if n < 1 or rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rope_tables: n={n} rotary_dim={rotary_dim}")
@@ -1454,7 +1455,9 @@ def paged_attn(q, kcache, vcache, table, lens, slopes=None, cu_rows=None, max_ro
     softmax(scale * q.k + slope_h * (j - i)) v; slopes [Hq] fp32 (ALiBi) or None; scale defaults to dh^-1/2.
     Hq a multiple of Hkv: query head h reads head h // (Hq // Hkv).  Rows that see nothing get zeros; what masked slots
     hold has no effect.  max_rows, max_len: upper bounds of n_b and lens[b], known on the host, that shape the launch
-    (defaults: all rows, the table's width; a wrong one costs time, not results).  Returns a dense tensor of q's shape."""
+    (defaults: all rows, the table's width; a wrong one costs time, not results beyond their last bits).  Softmax, sums and
+    joins are fp32; in bf16 the weights enter the product with v with 15 bits or more where a workgroup has few rows, as
+    bf16 values (8 bits) where it has more than 32, as in the training attention.  Returns a dense tensor of q's shape."""
     name = "paged_attn"
     if not q.is_cuda:
         raise RuntimeError(f"{name}: musicgeneration_amd runs on the GPU only (q is on {q.device}); there is no CPU fallback")
